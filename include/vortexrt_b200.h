@@ -147,8 +147,9 @@ VRT_API int vrt_lm_head_argmax(vrt_ctx* ctx, const void* d_weights, uint64_t wei
                                void* stream);
 
 /* Device error word of the pipeline entry points above (bit 0: a bounded
- * wait of the staged mat-vec kernel for its own bulk copy gave up, after
- * about a second; that call's outputs are then undefined), read and cleared.
+ * wait of a kernel for its own copies gave up, after about a second; that
+ * call's outputs are then undefined; bit 5: a vrt_kv8_* call met a length, an
+ * offset or a page outside its arrays), read and cleared.
  * ctx != NULL: the context's calls (its stream is synchronised first);
  * ctx == NULL: vrt_q8_ffn_static's calls on the current device (synchronise
  * the stream they ran on first).  No counterpart in the reference, whose
@@ -211,6 +212,100 @@ VRT_API int vrt_q8m_gemm_gelu(vrt_ctx* ctx, const void* d_q8m_pair, uint32_t ffn
 /* LM head + argmax over a packed vocab matrix (logits written when d_logits != NULL). */
 VRT_API int vrt_q8t_lm_head_argmax(vrt_ctx* ctx, const void* d_packed, uint32_t vocab, uint32_t cols,
                                    const float* d_x, float* d_logits, vrt_argmax_result* d_out, void* stream);
+
+/* ------------------------------------------------- paged 8-bit KV cache
+ * Keys and values of many sequences in pages of VRT_KV8_PAGE tokens, one int8
+ * code a value and one fp32 scale for each (page, KV head), K and V apart: a
+ * quarter of an fp32 cache.  For the rows x that a page holds so far
+ *     scale = fl32(max|x| / 127),  code = x / scale rounded half to even,
+ * so a page's contents depend on its tokens alone and not on the calls that
+ * brought them: the rows of a page that is not full are also kept as given
+ * (the tail), and the page is quantised again from them as rows join.  A page
+ * and head with a non-finite value has scale NaN (all its values read NaN).
+ *
+ * All arrays are the caller's device memory on the context's device; the
+ * calls allocate nothing, keep nothing and are asynchronous on `stream`
+ * (capturable).  Lengths, offsets and the page table are read on the device
+ * when the call runs.  A length beyond the table's row (or beyond max_len),
+ * more rows than max_new, or a page id outside the pool is clamped, or that
+ * page left out, and bit 5 of vrt_pipeline_status is set: nothing outside
+ * the arrays is touched.  Two sequences of one call must not append to the
+ * same page; reading shared pages is fine.  No counterpart in the reference,
+ * whose cache is fp32 and contiguous (src/gemma3.cpp:1590-1600). */
+#define VRT_KV8_PAGE 32
+
+/* Element type of rows given to and taken from the cache (q, k, v, out). */
+enum { VRT_F32 = 0, VRT_F16 = 1, VRT_BF16 = 2 };
+
+typedef struct {
+    uint32_t kv_heads;      /* >= 1                                        */
+    uint32_t head_dim;      /* 64, 128 or 256                              */
+    uint32_t pages;         /* pages in the pool                           */
+    uint32_t max_seqs;      /* rows of the page table and of the tails     */
+    uint32_t pages_per_seq; /* entries of one row of the page table        */
+    int dtype;              /* VRT_F32 / VRT_F16 / VRT_BF16                */
+    int8_t* d_k;            /* [pages][kv_heads][VRT_KV8_PAGE][head_dim]   */
+    int8_t* d_v;            /* [pages][kv_heads][head_dim][VRT_KV8_PAGE]: a page's tokens side by side */
+    float* d_k_scale;       /* [pages][kv_heads]                           */
+    float* d_v_scale;
+    void* d_k_tail;         /* [max_seqs][kv_heads][VRT_KV8_PAGE][head_dim] of dtype */
+    void* d_v_tail;
+    const int32_t* d_table; /* [max_seqs][pages_per_seq]: pool index of each page of a sequence */
+} vrt_kv8_cache;
+
+/* Which keys a query sees and what becomes of its scores.  The query of
+ * position p sees key t < len when t < prefix, or when t <= p and (window ==
+ * 0 or p - t < window).  A prefix is thus seen by every query whatever the
+ * order and the window (an image's tokens, the first tokens that a sliding
+ * window keeps in sight).  s = scale * q.k, then softcap * tanh(s / softcap)
+ * when softcap > 0.  A query that sees nothing gives zeros and lse = -inf. */
+typedef struct {
+    uint32_t heads;          /* query heads: 1 to 8 for each KV head        */
+    float scale;
+    float softcap;           /* 0 = none                                    */
+    uint32_t window;         /* 0 = none                                    */
+    const int32_t* d_prefix; /* [count], or NULL = 0 for all                */
+} vrt_kv8_attn;
+
+/* Append rows [d_cu[i], d_cu[i+1]) of d_k / d_v ([rows][kv_heads][head_dim],
+ * consecutive rows row_stride elements apart; 0 = packed) to sequence i, which
+ * holds d_start[i] tokens, for i < count.  d_cu NULL: one row each.  max_new:
+ * the most rows of one sequence.  Rows must start on 16-byte boundaries. */
+VRT_API int vrt_kv8_append(vrt_ctx* ctx, const vrt_kv8_cache* cache, const void* d_k, const void* d_v,
+                           uint64_t row_stride, const int32_t* d_start, const int32_t* d_cu, uint32_t count,
+                           uint32_t max_new, void* stream);
+
+/* Values that the cache stands for: tokens d_start[i] + [0, d_cu[i+1] -
+ * d_cu[i]) of sequence i -> fp32 rows [d_cu[i], d_cu[i+1]) of d_k_out and
+ * d_v_out ([rows][kv_heads][head_dim], packed).  d_cu NULL: one row each.
+ * Rows of a page outside the pool are left as they were. */
+VRT_API int vrt_kv8_read(vrt_ctx* ctx, const vrt_kv8_cache* cache, const int32_t* d_start, const int32_t* d_cu,
+                         uint32_t count, uint32_t max_rows, float* d_k_out, float* d_v_out, void* stream);
+
+/* Bytes of workspace that vrt_kv8_decode (max_new = 1) or vrt_kv8_prefill
+ * need for these sizes (16-byte aligned, contents of no matter, the caller's;
+ * calls that may overlap on the GPU need one each). */
+VRT_API int vrt_kv8_workspace(vrt_ctx* ctx, const vrt_kv8_cache* cache, uint32_t heads, uint32_t count,
+                              uint32_t max_new, uint32_t max_len, uint64_t* bytes);
+
+/* Attention of one query token for each of `count` sequences: row i of d_q
+ * ([count][heads][head_dim], rows q_stride elements apart, 0 = packed) is the
+ * last of the d_len[i] tokens that sequence i holds.  max_len: no length is
+ * above it.  d_out like d_q (out_stride); d_lse [count][heads] or NULL.
+ * Rows must start on 16-byte boundaries.  A length of 0 gives zeros. */
+VRT_API int vrt_kv8_decode(vrt_ctx* ctx, const vrt_kv8_cache* cache, const vrt_kv8_attn* attn, const void* d_q,
+                           uint64_t q_stride, const int32_t* d_len, uint32_t count, uint32_t max_len, void* d_out,
+                           uint64_t out_stride, float* d_lse, void* d_workspace, uint64_t workspace_bytes,
+                           void* stream);
+
+/* The same for the last d_cu[i+1] - d_cu[i] tokens of each sequence (rows
+ * [d_cu[i], d_cu[i+1]) of d_q, d_out and d_lse), already appended: a prompt,
+ * or a chunk of one behind its history.  Rows behind the last sequence stay
+ * as they were. */
+VRT_API int vrt_kv8_prefill(vrt_ctx* ctx, const vrt_kv8_cache* cache, const vrt_kv8_attn* attn, const void* d_q,
+                            uint64_t q_stride, const int32_t* d_len, const int32_t* d_cu, uint32_t count,
+                            uint32_t max_new, uint32_t max_len, void* d_out, uint64_t out_stride, float* d_lse,
+                            void* d_workspace, uint64_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------ model */
 

@@ -67,6 +67,17 @@ class TpShard(C.Structure):
                                           "vocab")]
 
 
+class Kv8CacheStruct(C.Structure):
+    _fields_ = [(n, C.c_uint32) for n in ("kv_heads", "head_dim", "pages", "max_seqs", "pages_per_seq")] + [
+        ("dtype", C.c_int)] + [(n, C.c_void_p) for n in ("d_k", "d_v", "d_k_scale", "d_v_scale", "d_k_tail", "d_v_tail",
+                                                         "d_table")]
+
+
+class Kv8AttnStruct(C.Structure):
+    _fields_ = [("heads", C.c_uint32), ("scale", C.c_float), ("softcap", C.c_float), ("window", C.c_uint32),
+                ("d_prefix", C.c_void_p)]
+
+
 class ArgmaxResult(C.Structure):
     _fields_ = [("index", C.c_uint32), ("value", C.c_float)]
 
@@ -106,6 +117,11 @@ _SIGS = {
     "vrt_q8t_ffn": (_i, [_vp, _vp, _vp, _u32, _u32, _u32, _vp, _vp, _vp, _vp]),
     "vrt_q8t_lm_head_argmax": (_i, [_vp, _vp, _u32, _u32, _vp, _vp, _vp, _vp]),
     "vrt_q8t_gemm": (_i, [_vp, _vp, _u32, _u32, _vp, _u32, _vp, _vp]),
+    "vrt_kv8_append": (_i, [_vp, _vp, _vp, _vp, _u64, _vp, _vp, _u32, _u32, _vp]),
+    "vrt_kv8_read": (_i, [_vp, _vp, _vp, _vp, _u32, _u32, _vp, _vp, _vp]),
+    "vrt_kv8_workspace": (_i, [_vp, _vp, _u32, _u32, _u32, _u32, C.POINTER(_u64)]),
+    "vrt_kv8_decode": (_i, [_vp, _vp, _vp, _vp, _u64, _vp, _u32, _u32, _vp, _u64, _vp, _vp, _u64, _vp]),
+    "vrt_kv8_prefill": (_i, [_vp, _vp, _vp, _vp, _u64, _vp, _vp, _u32, _u32, _u32, _vp, _u64, _vp, _vp, _u64, _vp]),
     "vrt_batch_create": (_i, [_vp, _u32, _u32, _i, _vp]),
     "vrt_batch_destroy": (_i, [_vp]),
     "vrt_batch_prefill": (_i, [_vp, _u32, _vp, _u32]),
@@ -373,6 +389,85 @@ class Batch:
         out = np.zeros(count, np.uint32) if out is None else out
         check(lib().vrt_batch_last_ids(self.h, count, _ptr(out)))
         return out
+
+
+KV8_PAGE = 32
+
+
+class Kv8Cache:
+    """A paged 8-bit KV cache (vrt_kv8_*): the layout and the calls' meaning
+    stand in vortexrt_b200.h.  Arrays that are not given (device pointers as
+    ints) are allocated from the context and freed by close(); a table made
+    here is filled with set_table().  Row arguments are device pointers too."""
+
+    DTYPES = {"f32": 0, "f16": 1, "bf16": 2}
+
+    def __init__(self, ctx: Context, kv_heads: int, head_dim: int, pages: int, max_seqs: int, pages_per_seq: int,
+                 dtype: str = "f32", *, k: int | None = None, v: int | None = None, k_scale: int | None = None,
+                 v_scale: int | None = None, k_tail: int | None = None, v_tail: int | None = None,
+                 table: int | None = None):
+        self.ctx = ctx
+        self._own: list[int] = []
+        if dtype not in self.DTYPES:
+            raise VrtError(VRT_E_INVALID, f"kv8: unknown dtype {dtype!r}")
+        size = 4 if dtype == "f32" else 2
+        codes, scales = pages * kv_heads * KV8_PAGE * head_dim, pages * kv_heads * 4
+        tail = max_seqs * kv_heads * KV8_PAGE * head_dim * size
+        p = [self._array(a, n) for a, n in ((k, codes), (v, codes), (k_scale, scales), (v_scale, scales),
+                                            (k_tail, tail), (v_tail, tail), (table, max_seqs * pages_per_seq * 4))]
+        self.s = Kv8CacheStruct(kv_heads, head_dim, pages, max_seqs, pages_per_seq, self.DTYPES[dtype], *p)
+        self._ref = C.byref(self.s)
+
+    def _array(self, given: int | None, nbytes: int) -> int:
+        if given is not None:
+            return given
+        p = self.ctx.alloc(max(int(nbytes), 1))
+        self._own.append(p)
+        return p
+
+    def close(self):
+        own, self._own = self._own, []
+        if self.ctx.h and not sys.is_finalizing():
+            for p in own:
+                self.ctx.free(p)
+
+    def set_table(self, table: np.ndarray):
+        t = np.ascontiguousarray(table, np.int32)
+        if t.shape != (self.s.max_seqs, self.s.pages_per_seq):
+            raise VrtError(VRT_E_INVALID, f"kv8: a table of {t.shape} for {self.s.max_seqs} x {self.s.pages_per_seq}")
+        check(lib().vrt_upload(self.ctx.h, self.s.d_table, _ptr(t), t.nbytes))
+
+    def append(self, k: int, v: int, start: int, count: int, *, cu: int | None = None, max_new: int = 1,
+               row_stride: int = 0, stream=None):
+        check(lib().vrt_kv8_append(self.ctx.h, self._ref, k, v, row_stride, start, cu, count, max_new, stream))
+
+    def read(self, start: int, count: int, k_out: int, v_out: int, *, cu: int | None = None, max_rows: int = 1,
+             stream=None):
+        check(lib().vrt_kv8_read(self.ctx.h, self._ref, start, cu, count, max_rows, k_out, v_out, stream))
+
+    def workspace_bytes(self, heads: int, count: int, max_new: int, max_len: int) -> int:
+        n = _u64()
+        check(lib().vrt_kv8_workspace(self.ctx.h, self._ref, heads, count, max_new, max_len, C.byref(n)))
+        return n.value
+
+    def _attention(self, heads, scale, softcap, window, prefix):
+        return C.byref(Kv8AttnStruct(heads, self.s.head_dim ** -0.5 if scale is None else scale, softcap, window, prefix))
+
+    def decode(self, q: int, lens: int, count: int, heads: int, out: int, *, max_len: int, scale: float | None = None,
+               softcap: float = 0.0, window: int = 0, prefix: int | None = None, lse: int | None = None,
+               q_stride: int = 0, out_stride: int = 0, workspace: int | None = None, workspace_bytes: int = 0,
+               stream=None):
+        check(lib().vrt_kv8_decode(self.ctx.h, self._ref, self._attention(heads, scale, softcap, window, prefix), q,
+                                   q_stride, lens, count, max_len, out, out_stride, lse, workspace, workspace_bytes,
+                                   stream))
+
+    def prefill(self, q: int, lens: int, cu: int, count: int, heads: int, out: int, *, max_new: int, max_len: int,
+                scale: float | None = None, softcap: float = 0.0, window: int = 0, prefix: int | None = None,
+                lse: int | None = None, q_stride: int = 0, out_stride: int = 0, workspace: int | None = None,
+                workspace_bytes: int = 0, stream=None):
+        check(lib().vrt_kv8_prefill(self.ctx.h, self._ref, self._attention(heads, scale, softcap, window, prefix), q,
+                                    q_stride, lens, cu, count, max_new, max_len, out, out_stride, lse, workspace,
+                                    workspace_bytes, stream))
 
 
 class Tokenizer:
