@@ -353,7 +353,12 @@ int attention(vrt_ctx* ctx, const vrt_kv8_cache* cache, const vrt_kv8_attn* attn
     p.status = status_word(ctx);
     DeviceScope dev(ctx->device);
     VRT_CUDA(dev.e);
-    VRT_CUDA(kv8_attention(p, cache->head_dim, cache->dtype, as_stream(ctx, stream)));
+    const int sms = ctx->prop.multiProcessorCount;
+    if (d_cu) {
+        VRT_CUDA(kv8_attention(p, cache->head_dim, cache->dtype, as_stream(ctx, stream)));
+    } else {
+        VRT_CUDA(kv8_decode(p, cache->head_dim, cache->dtype, sms, d_workspace, as_stream(ctx, stream)));
+    }
     return VRT_OK;
 }
 
@@ -424,7 +429,8 @@ int vrt_kv8_workspace(vrt_ctx* ctx, const vrt_kv8_cache* cache, uint32_t heads, 
     VRT_TRY(check_batch(cache, count, max_new, "max_new"));
     VRT_TRY(check_heads(cache, heads));
     if (!ctx) return fail(VRT_E_INVALID, "kv8: null context");
-    *bytes = 0;
+    const int sms = ctx->prop.multiProcessorCount;
+    *bytes = kv8_decode_workspace(sms, cache->head_dim, cache->kv_heads, heads, count, max_len);
     return VRT_OK;
 }
 

@@ -119,5 +119,7 @@ __host__ __device__ inline int64_t kv8_window_lo(int64_t pos, uint32_t window) {
 
 cudaError_t kv8_append(const Kv8Append& p, uint32_t hd, int dtype, uint32_t count, cudaStream_t s);
 cudaError_t kv8_attention(const Kv8Attn& p, uint32_t hd, int dtype, cudaStream_t s);
+cudaError_t kv8_decode(const Kv8Attn& p, uint32_t hd, int dtype, int sms, void* workspace, cudaStream_t s);
+uint64_t kv8_decode_workspace(int sms, uint32_t hd, uint32_t kv, uint32_t heads, uint32_t count, uint32_t max_len);
 
 }  // namespace vrt

@@ -1,0 +1,567 @@
+// Single-token attention over the paged 8-bit KV cache (kv8.cuh): one pass
+// over the visible pages, split over the GPU, joined by a second kernel.
+//
+// Bound by HBM: 2 * head_dim bytes a token and KV head, read once whatever
+// the number of query heads.  An int8 code is exact in fp16, so the products
+// run on mma.sync m16n8k16 (fp16 in, fp32 sums) with the page as the 16-row
+// operand and the query heads of one KV head as the 8 columns: no row of the
+// instruction is padding, where tcgen05 would take the 1..8 heads as 128
+// rows.  The tensor work is far below its peak (11 SM cycles of HBM time for
+// one mma at 6.4 TB/s), so what counts is bytes in flight.
+//
+// CTA (split, KV head, sequence): 4 warps, each with its own ring of bulk
+// copies (24 KB a warp, two CTAs an SM: 192 KB in flight); page j of the
+// split belongs to warp j % 4, its keys and its values are two ring items.
+//   scores  S^T[token][head] = K[token][dim] Q^T[dim][head]: the 16-byte piece
+//           of a key row that a lane holds is 4 k-steps of its A fragment,
+//           the dims are permuted alike in Q's fragments;
+//   softmax running maximum and sum a head in registers, base 2;
+//   output  O^T[dim][head] += V^T[dim][token] P^T[token][head]: the value page
+//           lies [dim][token], so 8 bytes of a lane are again A fragments; P
+//           goes from the accumulator layout to the operand layout by
+//           movmatrix, with the page's tokens dealt to rows so that it fits.
+// A page's products start from zero and join the fp32 sums by one FMA with
+// the page's value scale: the tensor core cuts its sums at every step, which
+// would add up over a long history.
+//
+// Operands: a query row is brought to [2^14, 2^15) by a power of two, then
+// fp16 (exact for f16 and bf16 rows) or, for f32 rows, fp16 + fp16 remainder
+// (22 bits).  Weights are 2^14 exp(s - maximum) in fp16: half a step is 2^-11
+// of a weight (averaged over the keys below half a step of a 16-bit output),
+// and what falls under fp16's smallest step is 2^-39 of the largest weight;
+// for f32 rows fp16 + fp16 remainder.  The remainders take columns 4..7 when
+// there are at most 4 heads, a second mma otherwise.
+
+#include <cuda_runtime.h>
+
+#include <mutex>
+
+#include "kv8.cuh"
+
+namespace vrt {
+
+constexpr int kKdWarps = 4;
+constexpr int kKdThreads = kKdWarps * 32;
+constexpr uint32_t kKdRing = 24 * 1024;  // bytes of ring of one warp
+constexpr uint32_t kKdMaxSplits = 128;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kKdLift = 14.0f;  // weights are held times 2^14
+
+template <int HD>
+struct KdShape {
+    static constexpr uint32_t kItem = kKv8Page * HD;   // bytes of one page of one head: a ring item
+    static constexpr int kItems = kKdRing / kItem;     // 12, 6 or 3
+    static constexpr int kSteps = HD / 16;             // k-steps of the scores, row tiles of the output
+};
+
+struct KdParams {
+    Kv8Attn a;
+    uint32_t chunk;   // pages of one split, a multiple of the warps
+    uint32_t splits;  // grid.x
+    float* part;      // [count][H][splits][head_dim] unnormalised outputs
+    float* part_ml;   // [count][H][splits][2] maximum (base 2) and sum
+};
+
+// Visible pages of one sequence's newest token: [0, a) and [b0, b1).
+struct KdSpan {
+    int64_t len, lo, prefix;
+    uint32_t a, b0, b1;
+    __device__ __forceinline__ uint32_t count() const { return a + b1 - b0; }
+    __device__ __forceinline__ uint32_t page(uint32_t i) const { return i < a ? i : b0 + i - a; }
+};
+
+__device__ __forceinline__ KdSpan kd_span(const Kv8Attn& p, uint32_t seq) {
+    KdSpan s;
+    const int64_t limit = min(static_cast<int64_t>(p.max_len), static_cast<int64_t>(p.c.pps) * kKv8Page);
+    const int64_t len = p.len[seq];
+    if (len < 0 || len > limit) atomicOr(p.status, kStatusKv8Range);
+    s.len = max(static_cast<int64_t>(0), min(len, limit));
+    s.lo = kv8_window_lo(s.len - 1, p.window);
+    s.prefix = p.prefix ? max(static_cast<int64_t>(0), min(static_cast<int64_t>(p.prefix[seq]), s.len)) : 0;
+    s.a = static_cast<uint32_t>((s.prefix + kKv8Page - 1) / kKv8Page);
+    s.b1 = static_cast<uint32_t>((s.len + kKv8Page - 1) / kKv8Page);
+    s.b0 = min(s.b1, max(s.a, static_cast<uint32_t>(s.lo / kKv8Page)));
+    return s;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b.x), "r"(b.y));
+}
+
+__device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+// Codes 0, 1 (lo) or 2, 3 (hi) of a word whose bytes were offset by 128, as
+// two fp16: the byte under the exponent of 1024, less 1024 + 128.
+__device__ __forceinline__ uint32_t codes_lo(uint32_t w) {
+    const uint32_t b = __byte_perm(w, 0x64646464u, 0x4140u);
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&b), __float2half2_rn(1152.0f));
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
+    const uint32_t b = __byte_perm(w, 0x64646464u, 0x4342u);
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&b), __float2half2_rn(1152.0f));
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ uint32_t pack_half(__half a, __half b) {
+    return static_cast<uint32_t>(__half_as_ushort(a)) | static_cast<uint32_t>(__half_as_ushort(b)) << 16;
+}
+
+// softcap * tanh(x / softcap), in base-2 units.  f32 rows take tanhf; for 16-bit
+// rows 1 - 2 / (1 + e^2y) is off by some 2^-22 of the cap, far below a weight's rounding.
+template <bool EXACT>
+__device__ __forceinline__ float capped(float x, float cap, float inv_cap) {
+    if (EXACT) return cap * tanhf(x * inv_cap) * kLog2e;
+    const float e = ex2(x * inv_cap * (2.0f * kLog2e));
+    return cap * kLog2e * (1.0f - __fdividef(2.0f, e + 1.0f));
+}
+
+// TERMS: fp16 terms of an operand (2 for f32 rows).  SETS: mma of each step
+// (2: more than 4 heads with remainders).
+template <typename T, int HD, int TERMS, int SETS>
+__global__ void __launch_bounds__(kKdThreads, 2) kv8_decode_kernel(const KdParams p) {
+    using Shape = KdShape<HD>;
+    constexpr bool kPacked = TERMS == 2 && SETS == 1;  // columns 4..7 are the remainders of heads 0..3
+    constexpr int D = Shape::kItems, KS = Shape::kSteps;
+    extern __shared__ __align__(128) uint8_t sm[];
+    uint2* qf = reinterpret_cast<uint2*>(sm + kKdWarps * kKdRing);        // [SETS][KS][32] query fragments
+    uint64_t* bars = reinterpret_cast<uint64_t*>(qf + SETS * KS * 32);    // [warps][D]
+    float* q_unit = reinterpret_cast<float*>(bars + kKdWarps * D);        // [8] what a query row was divided by
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t4 = lane & 3;
+    const uint32_t split = blockIdx.x, g = blockIdx.y, seq = blockIdx.z, R = p.a.H / p.a.c.kv;
+    pdl_trigger();
+    const KdSpan span = kd_span(p.a, seq);
+    const uint32_t n = span.count(), j0 = split * p.chunk;
+    if (j0 >= n && !(split == 0 && n == 0)) return;
+    const uint32_t j1 = min(n, j0 + p.chunk);
+
+    uint64_t* bar = bars + warp * D;
+    uint8_t* ring = sm + warp * kKdRing;
+    if (lane < D) mbar_init(bar + lane, 1);
+    fence_mbar_init();
+    __syncwarp();
+
+    // This warp's pages: j0 + warp + 4 i for i < mine.  Lane l knows page l of
+    // the current group of 32: pool index and scales.
+    const uint32_t mine = j0 + warp < j1 ? (j1 - j0 - warp + kKdWarps - 1) / kKdWarps : 0;
+    const int64_t kv = p.a.c.kv;
+    auto look_up = [&](uint32_t i, int& id, float& ks, float& vs) {
+        id = 0;
+        ks = vs = 0.0f;
+        if (i >= mine) return;
+        id = kv8_page(p.a.c, seq, span.page(j0 + warp + kKdWarps * i), p.a.status);
+        if (id < 0) return;
+        ks = __ldg(p.a.c.k_scale + id * kv + g);
+        vs = __ldg(p.a.c.v_scale + id * kv + g);
+    };
+    int id_now, id_next = 0;
+    float ks_now, vs_now, ks_next = 0.0f, vs_next = 0.0f;
+    look_up(lane, id_now, ks_now, vs_now);
+    if (mine > 32) look_up(32 + lane, id_next, ks_next, vs_next);
+    uint32_t issued = 0;  // ring items asked for: keys of page i are item 2 i, values 2 i + 1
+    auto issue = [&](uint32_t base) {  // base: first page of id_now's group
+        const uint32_t i = issued / 2;
+        const int id = i - base < 32 ? __shfl_sync(0xffffffffu, id_now, i - base)
+                                     : __shfl_sync(0xffffffffu, id_next, i - base - 32);
+        if (lane == 0) {
+            const uint64_t at = (static_cast<uint64_t>(id < 0 ? 0 : id) * kv + g) * Shape::kItem;
+            uint64_t* b = bar + issued % D;
+            mbar_arrive_expect_tx(b, Shape::kItem);
+            bulk_copy_g2s(ring + issued % D * Shape::kItem, (issued & 1 ? p.a.c.v : p.a.c.k) + at, Shape::kItem, b);
+        }
+        ++issued;
+    };
+    while (issued < 2 * mine && issued < D) issue(0);
+
+    // query fragments: lane (g8, t4) of step (c, s) holds dims 64 c + 16 t4 + 4 s + 0..3 of head g8
+    {
+        const uint32_t h = tid / 16, piece = tid % 16;  // 16 threads a head, HD / 16 dims each
+        constexpr int E = HD / 16;
+        float x[E], m = 0.0f;
+        const T* q = static_cast<const T*>(p.a.q) + static_cast<uint64_t>(seq) * p.a.q_stride +
+                     static_cast<uint64_t>(g * R + h) * HD + piece * E;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            x[e] = h < R ? to_f32(q[e]) : 0.0f;
+            m = fmaxf(m, fabsf(x[e]));
+        }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        // 2^(14 - exponent of the largest), within the normal numbers
+        const int ex = static_cast<int>(__float_as_uint(m) >> 23);
+        const int up = m > 0.0f && ex < 255 ? max(-126, min(126, 14 - (ex - 127))) : 0;
+        const float mul = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
+        if (piece == 0) q_unit[h] = 1.0f / mul;
+        __half* f = reinterpret_cast<__half*>(qf);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int d = piece * E + e;
+            const int step = d / 64 * 4 + d % 16 / 4, t = d % 64 / 16;
+            const int at = ((step * 32 + static_cast<int>(h) * 4 + t) * 4) + d % 4;
+            __half hi, lo;
+            split_f16(x[e] * mul, hi, lo);
+            if (kPacked) {
+                if (h < 4) {
+                    f[at] = hi;
+                    f[at + 4 * 4 * 4] = lo;  // head h + 4
+                }
+            } else {
+                f[at] = hi;
+                if (SETS == 2) f[at + KS * 32 * 4] = lo;
+            }
+        }
+    }
+    __syncthreads();
+    const int head0 = kPacked ? (2 * t4) % 4 : 2 * t4;  // heads of this lane's two columns
+    const bool plain_cap = p.a.softcap > 0.0f;
+    const float unit = plain_cap ? 1.0f : kLog2e, inv_cap = plain_cap ? 1.0f / p.a.softcap : 0.0f;
+    const float sc[2] = {q_unit[head0] * (p.a.scale * unit), q_unit[head0 + 1] * (p.a.scale * unit)};
+
+    float acc[KS][4];
+#pragma unroll
+    for (int i = 0; i < KS; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][e] = 0.0f;
+    float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+    bool ok = true;
+    uint32_t used = 0;  // ring items consumed
+    auto refill = [&](uint32_t base) {
+        ++used;
+        __syncwarp();
+        if (issued < 2 * mine) issue(base);
+    };
+
+    for (uint32_t i = 0; i < mine; ++i) {
+        const uint32_t base = i & ~31u;
+        if (i == base && i) {
+            id_now = id_next;
+            ks_now = ks_next;
+            vs_now = vs_next;
+            look_up(base + 32 + lane, id_next, ks_next, vs_next);
+        }
+        const float ks = __shfl_sync(0xffffffffu, ks_now, i & 31), vs = __shfl_sync(0xffffffffu, vs_now, i & 31);
+        const bool there = __shfl_sync(0xffffffffu, id_now, i & 31) >= 0;
+        const int64_t t0 = static_cast<int64_t>(span.page(j0 + warp + kKdWarps * i)) * kKv8Page;
+
+        // ---- scores: block b of 8 rows holds tokens 8 (row / 2) + row % 2 + 2 b
+        ok &= mbar_wait_bounded(bar + used % D, (used / D) & 1);
+        float s[2][4];
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[m][e] = 0.0f;
+        {
+            const uint8_t* kp = ring + used % D * Shape::kItem + (8 * (g8 >> 1) + (g8 & 1)) * HD + t4 * 16;
+#pragma unroll
+            for (int c = 0; c < HD / 64; ++c) {
+                uint32_t w[4][4];
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const uint4 u = *reinterpret_cast<const uint4*>(kp + 2 * b * HD + 64 * c);
+                    w[b][0] = u.x ^ 0x80808080u;
+                    w[b][1] = u.y ^ 0x80808080u;
+                    w[b][2] = u.z ^ 0x80808080u;
+                    w[b][3] = u.w ^ 0x80808080u;
+                }
+#pragma unroll
+                for (int st = 0; st < 4; ++st) {
+                    const uint2 q0 = qf[(c * 4 + st) * 32 + lane];
+                    uint2 q1;
+                    if (SETS == 2) q1 = qf[(KS + c * 4 + st) * 32 + lane];
+#pragma unroll
+                    for (int m = 0; m < 2; ++m) {
+                        const uint32_t a0 = codes_lo(w[2 * m][st]), a1 = codes_lo(w[2 * m + 1][st]);
+                        const uint32_t a2 = codes_hi(w[2 * m][st]), a3 = codes_hi(w[2 * m + 1][st]);
+                        if (SETS == 2) mma_f16(s[m], a0, a1, a2, a3, q1);
+                        mma_f16(s[m], a0, a1, a2, a3, q0);
+                    }
+                }
+            }
+        }
+        refill(base);
+        if (kPacked) {
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[m][e] += __shfl_xor_sync(0xffffffffu, s[m][e], 2);
+        }
+        // ---- softmax: s[m][2 r + h] is block 2 m + r, this lane's head h
+        float top[2] = {mx[0], mx[1]};
+        const bool full = there && (t0 + 32 <= span.prefix || (t0 >= span.lo && t0 + 32 <= span.len));
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int64_t t = t0 + 8 * (g8 >> 1) + (g8 & 1) + 2 * b;
+            const bool see = full || (there && (t < span.prefix || (t >= span.lo && t < span.len)));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float& z = s[b >> 1][2 * (b & 1) + h];
+                z = z * ks * sc[h];
+                if (plain_cap) z = capped<TERMS == 2>(z, p.a.softcap, inv_cap);
+                if (!see) z = -INFINITY;
+                top[h] = fmaxf(top[h], z);
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], o));
+        }
+        if (__any_sync(0xffffffffu, top[0] != mx[0] || top[1] != mx[1])) {
+            float f[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                f[h] = mx[h] == -INFINITY ? 0.0f : ex2(mx[h] - top[h]);
+                sum[h] *= f[h];
+                mx[h] = top[h];
+            }
+#pragma unroll
+            for (int q = 0; q < KS; ++q)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[q][e] *= f[e & 1];
+        }
+        const float m0[2] = {mx[0] == -INFINITY ? 0.0f : mx[0] - kKdLift, mx[1] == -INFINITY ? 0.0f : mx[1] - kKdLift};
+        uint32_t ph[4], pl[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            __half hi[2], lo[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                // a score that was left out is -inf, whatever its scale: weight 0; a NaN stays
+                const float w = ex2(s[b >> 1][2 * (b & 1) + h] - m0[h]);
+                sum[h] += w;
+                if (TERMS == 2) {
+                    split_f16(w, hi[h], lo[h]);
+                } else {
+                    hi[h] = __float2half_rn(w);
+                }
+            }
+            ph[b] = pack_half(hi[0], hi[1]);
+            if (TERMS == 2) pl[b] = pack_half(lo[0], lo[1]);
+            if (kPacked && t4 >= 2) ph[b] = pl[b];
+            ph[b] = movmatrix(ph[b]);
+            if (SETS == 2) pl[b] = movmatrix(pl[b]);
+        }
+        // ---- output
+        ok &= mbar_wait_bounded(bar + used % D, (used / D) & 1);
+        {
+            const uint8_t* vp = ring + used % D * Shape::kItem + g8 * kKv8Page + t4 * 8;
+#pragma unroll
+            for (int q = 0; q < KS; ++q) {
+                uint2 u0 = *reinterpret_cast<const uint2*>(vp + q * 16 * kKv8Page);
+                uint2 u1 = *reinterpret_cast<const uint2*>(vp + (q * 16 + 8) * kKv8Page);
+                u0.x ^= 0x80808080u;
+                u0.y ^= 0x80808080u;
+                u1.x ^= 0x80808080u;
+                u1.y ^= 0x80808080u;
+                float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const uint32_t a0 = codes_lo(u0.x), a1 = codes_lo(u1.x), a2 = codes_hi(u0.x), a3 = codes_hi(u1.x);
+                const uint32_t c0 = codes_lo(u0.y), c1 = codes_lo(u1.y), c2 = codes_hi(u0.y), c3 = codes_hi(u1.y);
+                if (SETS == 2) {
+                    mma_f16(o, a0, a1, a2, a3, make_uint2(pl[0], pl[1]));
+                    mma_f16(o, c0, c1, c2, c3, make_uint2(pl[2], pl[3]));
+                }
+                mma_f16(o, a0, a1, a2, a3, make_uint2(ph[0], ph[1]));
+                mma_f16(o, c0, c1, c2, c3, make_uint2(ph[2], ph[3]));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[q][e] = fmaf(o[e], vs, acc[q][e]);
+            }
+        }
+        refill(base);
+    }
+    if (!ok && lane == 0) atomicOr(p.a.status, kStatusWaitTimeout);
+
+    // ---- join the warps: [warp][column][HD] outputs over the rings, then maxima and sums
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], o);
+    }
+    __syncthreads();
+    float* wo = reinterpret_cast<float*>(sm);
+    float* wm = reinterpret_cast<float*>(qf);  // [warp][8][2]
+#pragma unroll
+    for (int q = 0; q < KS; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) wo[(warp * 8 + 2 * t4 + (e & 1)) * HD + q * 16 + g8 + 8 * (e >> 1)] = acc[q][e];
+    if (g8 == 0 && (!kPacked || t4 < 2)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            wm[(warp * 8 + 2 * t4 + h) * 2] = mx[h] - kKdLift;  // sums are times 2^14
+            wm[(warp * 8 + 2 * t4 + h) * 2 + 1] = sum[h];
+        }
+    }
+    __syncthreads();
+    const bool alone = n <= p.chunk;  // the sequence's only split
+    for (uint32_t r = warp; r < R; r += kKdWarps) {
+        float m = -INFINITY, l = 0.0f, f[kKdWarps];
+#pragma unroll
+        for (int w = 0; w < kKdWarps; ++w) m = fmaxf(m, wm[(w * 8 + r) * 2]);
+#pragma unroll
+        for (int w = 0; w < kKdWarps; ++w) {
+            // a warp without pages has maximum -inf and sum 0; one whose scores are NaN has sum NaN
+            f[w] = wm[(w * 8 + r) * 2] == -INFINITY ? 1.0f : ex2(wm[(w * 8 + r) * 2] - m);
+            l += wm[(w * 8 + r) * 2 + 1] * f[w];
+        }
+        const uint64_t row = static_cast<uint64_t>(seq) * p.a.H + g * R + r;
+        float* part = p.part + (row * p.splits + split) * HD;
+        T* out = static_cast<T*>(p.a.out) + static_cast<uint64_t>(seq) * p.a.out_stride + static_cast<uint64_t>(g * R + r) * HD;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        for (int d = lane; d < HD; d += 32) {
+            float v = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kKdWarps; ++w) {
+                float x = wo[(w * 8 + r) * HD + d];
+                if (kPacked) x += wo[(w * 8 + r + 4) * HD + d];
+                v = fmaf(x, f[w], v);
+            }
+            if (alone) {
+                out[d] = from_f32<T>(v * inv);
+            } else {
+                part[d] = v;
+            }
+        }
+        if (lane == 0) {
+            if (alone) {
+                if (p.a.lse) p.a.lse[row] = l == 0.0f ? -INFINITY : (m == -INFINITY ? l : m / kLog2e + logf(l));
+            } else {
+                p.part_ml[(row * p.splits + split) * 2] = m;
+                p.part_ml[(row * p.splits + split) * 2 + 1] = l;
+            }
+        }
+    }
+}
+
+constexpr int kKjThreads = 256;
+
+// CTA (head, sequence): the splits' outputs in split order, 8 warps over the
+// splits, then over each other.
+template <typename T, int HD>
+__global__ void __launch_bounds__(kKjThreads) kv8_decode_join_kernel(const KdParams p) {
+    constexpr int W = kKjThreads / 32;
+    __shared__ float f[kKdMaxSplits];
+    __shared__ float o[W][HD];
+    __shared__ float total;
+    const uint32_t h = blockIdx.x, seq = blockIdx.y;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    pdl_wait();
+    const uint32_t n = kd_span(p.a, seq).count();
+    if (n <= p.chunk) return;  // the only split wrote the output itself
+    const uint32_t used = (n + p.chunk - 1) / p.chunk;
+    const uint64_t row = static_cast<uint64_t>(seq) * p.a.H + h;
+    const float* ml = p.part_ml + row * p.splits * 2;
+    if (warp == 0) {
+        float m = -INFINITY, l = 0.0f;
+        for (uint32_t i = lane; i < used; i += 32) m = fmaxf(m, ml[2 * i]);
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+        for (uint32_t i = lane; i < used; i += 32) {
+            f[i] = ml[2 * i] == -INFINITY ? 1.0f : ex2(ml[2 * i] - m);
+            l += ml[2 * i + 1] * f[i];
+        }
+        l = warp_sum(l);
+        if (lane == 0) {
+            total = l;
+            if (p.a.lse) p.a.lse[row] = l == 0.0f ? -INFINITY : (m == -INFINITY ? l : m / kLog2e + logf(l));
+        }
+    }
+    __syncthreads();
+    const float* part = p.part + row * p.splits * HD;
+    float v[HD / 32];
+#pragma unroll
+    for (int e = 0; e < HD / 32; ++e) v[e] = 0.0f;
+#pragma unroll 4
+    for (uint32_t i = warp; i < used; i += W) {
+#pragma unroll
+        for (int e = 0; e < HD / 32; ++e) v[e] = fmaf(part[static_cast<uint64_t>(i) * HD + lane + 32 * e], f[i], v[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < HD / 32; ++e) o[warp][lane + 32 * e] = v[e];
+    __syncthreads();
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    T* out = static_cast<T*>(p.a.out) + static_cast<uint64_t>(seq) * p.a.out_stride + static_cast<uint64_t>(h) * HD;
+    for (int d = threadIdx.x; d < HD; d += kKjThreads) {
+        float x = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) x += o[w][d];
+        out[d] = from_f32<T>(x * inv);
+    }
+}
+
+// ------------------------------------------------------------------- host
+
+// Pages of a split and splits of the longest sequence.  About four rounds of
+// the 2 CTAs that an SM holds, so that sequences of unlike length even out;
+// at least two pages a warp, below which starting a CTA costs more than its
+// pages.
+static void kd_plan(int sms, uint32_t kv, uint32_t count, uint32_t max_len, uint32_t& chunk, uint32_t& splits) {
+    const uint64_t pages = (static_cast<uint64_t>(max_len) + kKv8Page - 1) / kKv8Page;
+    const uint64_t want = std::max<uint64_t>(1, 8ull * sms / (static_cast<uint64_t>(kv) * std::max(1u, count)));
+    const uint64_t cap = std::min<uint64_t>(want, kKdMaxSplits);
+    uint64_t c = std::max<uint64_t>((pages + cap - 1) / cap, 2 * kKdWarps);
+    c = (c + kKdWarps - 1) / kKdWarps * kKdWarps;
+    chunk = static_cast<uint32_t>(c);
+    splits = static_cast<uint32_t>((pages + c - 1) / c);
+}
+
+uint64_t kv8_decode_workspace(int sms, uint32_t hd, uint32_t kv, uint32_t heads, uint32_t count, uint32_t max_len) {
+    uint32_t chunk, splits;
+    kd_plan(sms, kv, count, max_len, chunk, splits);
+    return splits > 1 ? static_cast<uint64_t>(count) * heads * splits * (hd + 2) * 4 : 0;
+}
+
+template <typename T, int HD, int TERMS, int SETS>
+static cudaError_t kd_launch(const KdParams& p, cudaStream_t s) {
+    using Shape = KdShape<HD>;
+    constexpr uint32_t smem = kKdWarps * kKdRing + SETS * Shape::kSteps * 32 * 8 + kKdWarps * Shape::kItems * 8 + 8 * 4;
+    static std::mutex mu;
+    static uint64_t done = 0;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    {
+        std::lock_guard<std::mutex> lock(mu);
+        const uint64_t bit = dev < 64 ? 1ull << dev : 0ull;
+        if (!(done & bit)) {
+            e = cudaFuncSetAttribute(kv8_decode_kernel<T, HD, TERMS, SETS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+            if (e != cudaSuccess) return e;
+            done |= bit;
+        }
+    }
+    e = launch(kv8_decode_kernel<T, HD, TERMS, SETS>, dim3(p.splits, p.a.c.kv, p.a.count), dim3(kKdThreads), smem, s, false, p);
+    if (e != cudaSuccess || p.splits == 1) return e;
+    return launch(kv8_decode_join_kernel<T, HD>, dim3(p.a.H, p.a.count), dim3(kKjThreads), 0, s, true, p);
+}
+
+cudaError_t kv8_decode(const Kv8Attn& a, uint32_t hd, int dtype, int sms, void* workspace, cudaStream_t s) {
+    KdParams p{};
+    p.a = a;
+    kd_plan(sms, a.c.kv, a.count, a.max_len, p.chunk, p.splits);
+    p.part = static_cast<float*>(workspace);
+    p.part_ml = p.part + static_cast<uint64_t>(a.count) * a.H * p.splits * hd;
+    const bool wide = a.H / a.c.kv > 4;
+#define VRT_KD(HD)                                                                              \
+    if (hd == HD) {                                                                             \
+        if (dtype == VRT_F16) return kd_launch<__half, HD, 1, 1>(p, s);                         \
+        if (dtype == VRT_BF16) return kd_launch<__nv_bfloat16, HD, 1, 1>(p, s);                 \
+        return wide ? kd_launch<float, HD, 2, 2>(p, s) : kd_launch<float, HD, 2, 1>(p, s);      \
+    }
+    VRT_KD(64) VRT_KD(128) VRT_KD(256)
+#undef VRT_KD
+    return cudaErrorInvalidValue;
+}
+
+}  // namespace vrt
