@@ -10,8 +10,8 @@
 // one mma at 6.4 TB/s), so what counts is bytes in flight.
 //
 // CTA (split, KV head, sequence): 4 warps, each with its own ring of bulk
-// copies (24 KB a warp, two CTAs an SM: 192 KB in flight); page j of the
-// split belongs to warp j % 4, its keys and its values are two ring items.
+// copies (192 KB an SM); page j of the split belongs to warp j % 4, its keys
+// and its values are two ring items.
 //   scores  S^T[token][head] = K[token][dim] Q^T[dim][head]: the 16-byte piece
 //           of a key row that a lane holds is 4 k-steps of its A fragment,
 //           the dims are permuted alike in Q's fragments;
@@ -42,7 +42,6 @@ namespace vrt {
 
 constexpr int kKdWarps = 4;
 constexpr int kKdThreads = kKdWarps * 32;
-constexpr uint32_t kKdRing = 24 * 1024;  // bytes of ring of one warp
 constexpr uint32_t kKdMaxSplits = 128;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kKdLift = 14.0f;  // weights are held times 2^14
@@ -50,7 +49,15 @@ constexpr float kKdLift = 14.0f;  // weights are held times 2^14
 template <int HD>
 struct KdShape {
     static constexpr uint32_t kItem = kKv8Page * HD;   // bytes of one page of one head: a ring item
-    static constexpr int kItems = kKdRing / kItem;     // 12, 6 or 3
+    // Warps resident on an SM are what the dependent steps of a page need most
+    // (8x32768 f16: 8 warps an SM 224 us, 16 warps 175-181 us), then CTAs
+    // small enough that one starts while others stream (32x2304 bf16, 16
+    // warps: 2 CTAs 66 us, 4 CTAs 62 us).  At head_dim 256 the output
+    // accumulators allow 8 warps.
+    static constexpr int kCtas = HD == 256 ? 2 : 4;
+    static constexpr uint32_t kRing = 192 * 1024 / kCtas;
+    static constexpr int kItems = kRing / kItem / kKdWarps;  // 6, 3 or 3 items of ring a warp
+    static_assert(kRing % (kKdWarps * kItem) == 0, "a warp's ring holds whole items");
     static constexpr int kSteps = HD / 16;             // k-steps of the scores, row tiles of the output
 };
 
@@ -69,6 +76,11 @@ struct KdSpan {
     __device__ __forceinline__ uint32_t count() const { return a + b1 - b0; }
     __device__ __forceinline__ uint32_t page(uint32_t i) const { return i < a ? i : b0 + i - a; }
 };
+
+// The splits that a sequence of n visible pages uses (none longer than
+// `chunk`) and the pages of each: even shares.
+__device__ __forceinline__ uint32_t kd_used(uint32_t n, uint32_t chunk) { return n ? (n + chunk - 1) / chunk : 1u; }
+__device__ __forceinline__ uint32_t kd_share(uint32_t n, uint32_t used) { return (n + used - 1) / used; }
 
 __device__ __forceinline__ KdSpan kd_span(const Kv8Attn& p, uint32_t seq) {
     KdSpan s;
@@ -132,38 +144,39 @@ __device__ __forceinline__ float capped(float x, float cap, float inv_cap) {
 // TERMS: fp16 terms of an operand (2 for f32 rows).  SETS: mma of each step
 // (2: more than 4 heads with remainders).
 template <typename T, int HD, int TERMS, int SETS>
-__global__ void __launch_bounds__(kKdThreads, 2) kv8_decode_kernel(const KdParams p) {
+__global__ void __launch_bounds__(kKdThreads, KdShape<HD>::kCtas) kv8_decode_kernel(const KdParams p) {
     using Shape = KdShape<HD>;
     constexpr bool kPacked = TERMS == 2 && SETS == 1;  // columns 4..7 are the remainders of heads 0..3
-    constexpr int D = Shape::kItems, KS = Shape::kSteps;
+    constexpr int D = Shape::kItems, KS = Shape::kSteps, W = kKdWarps;
+    constexpr uint32_t kWarpRing = D * Shape::kItem;
     extern __shared__ __align__(128) uint8_t sm[];
-    uint2* qf = reinterpret_cast<uint2*>(sm + kKdWarps * kKdRing);        // [SETS][KS][32] query fragments
+    uint2* qf = reinterpret_cast<uint2*>(sm + Shape::kRing);        // [SETS][KS][32] query fragments
     uint64_t* bars = reinterpret_cast<uint64_t*>(qf + SETS * KS * 32);    // [warps][D]
-    float* q_unit = reinterpret_cast<float*>(bars + kKdWarps * D);        // [8] what a query row was divided by
+    float* q_unit = reinterpret_cast<float*>(bars + W * D);        // [8] what a query row was divided by
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t4 = lane & 3;
     const uint32_t split = blockIdx.x, g = blockIdx.y, seq = blockIdx.z, R = p.a.H / p.a.c.kv;
     pdl_trigger();
     const KdSpan span = kd_span(p.a, seq);
-    const uint32_t n = span.count(), j0 = split * p.chunk;
-    if (j0 >= n && !(split == 0 && n == 0)) return;
-    const uint32_t j1 = min(n, j0 + p.chunk);
+    const uint32_t n = span.count(), used_splits = kd_used(n, p.chunk), share = kd_share(n, used_splits);
+    if (split >= used_splits) return;
+    const uint32_t j0 = min(n, split * share), j1 = min(n, j0 + share);
 
     uint64_t* bar = bars + warp * D;
-    uint8_t* ring = sm + warp * kKdRing;
+    uint8_t* ring = sm + warp * kWarpRing;
     if (lane < D) mbar_init(bar + lane, 1);
     fence_mbar_init();
     __syncwarp();
 
     // This warp's pages: j0 + warp + 4 i for i < mine.  Lane l knows page l of
     // the current group of 32: pool index and scales.
-    const uint32_t mine = j0 + warp < j1 ? (j1 - j0 - warp + kKdWarps - 1) / kKdWarps : 0;
+    const uint32_t mine = j0 + warp < j1 ? (j1 - j0 - warp + W - 1) / W : 0;
     const int64_t kv = p.a.c.kv;
     auto look_up = [&](uint32_t i, int& id, float& ks, float& vs) {
         id = 0;
         ks = vs = 0.0f;
         if (i >= mine) return;
-        id = kv8_page(p.a.c, seq, span.page(j0 + warp + kKdWarps * i), p.a.status);
+        id = kv8_page(p.a.c, seq, span.page(j0 + warp + W * i), p.a.status);
         if (id < 0) return;
         ks = __ldg(p.a.c.k_scale + id * kv + g);
         vs = __ldg(p.a.c.v_scale + id * kv + g);
@@ -255,7 +268,7 @@ __global__ void __launch_bounds__(kKdThreads, 2) kv8_decode_kernel(const KdParam
         }
         const float ks = __shfl_sync(0xffffffffu, ks_now, i & 31), vs = __shfl_sync(0xffffffffu, vs_now, i & 31);
         const bool there = __shfl_sync(0xffffffffu, id_now, i & 31) >= 0;
-        const int64_t t0 = static_cast<int64_t>(span.page(j0 + warp + kKdWarps * i)) * kKv8Page;
+        const int64_t t0 = static_cast<int64_t>(span.page(j0 + warp + W * i)) * kKv8Page;
 
         // ---- scores: block b of 8 rows holds tokens 8 (row / 2) + row % 2 + 2 b
         ok &= mbar_wait_bounded(bar + used % D, (used / D) & 1);
@@ -405,13 +418,13 @@ __global__ void __launch_bounds__(kKdThreads, 2) kv8_decode_kernel(const KdParam
         }
     }
     __syncthreads();
-    const bool alone = n <= p.chunk;  // the sequence's only split
-    for (uint32_t r = warp; r < R; r += kKdWarps) {
-        float m = -INFINITY, l = 0.0f, f[kKdWarps];
+    const bool alone = used_splits == 1;
+    for (uint32_t r = warp; r < R; r += W) {
+        float m = -INFINITY, l = 0.0f, f[W];
 #pragma unroll
-        for (int w = 0; w < kKdWarps; ++w) m = fmaxf(m, wm[(w * 8 + r) * 2]);
+        for (int w = 0; w < W; ++w) m = fmaxf(m, wm[(w * 8 + r) * 2]);
 #pragma unroll
-        for (int w = 0; w < kKdWarps; ++w) {
+        for (int w = 0; w < W; ++w) {
             // a warp without pages has maximum -inf and sum 0; one whose scores are NaN has sum NaN
             f[w] = wm[(w * 8 + r) * 2] == -INFINITY ? 1.0f : ex2(wm[(w * 8 + r) * 2] - m);
             l += wm[(w * 8 + r) * 2 + 1] * f[w];
@@ -423,7 +436,7 @@ __global__ void __launch_bounds__(kKdThreads, 2) kv8_decode_kernel(const KdParam
         for (int d = lane; d < HD; d += 32) {
             float v = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kKdWarps; ++w) {
+            for (int w = 0; w < W; ++w) {
                 float x = wo[(w * 8 + r) * HD + d];
                 if (kPacked) x += wo[(w * 8 + r + 4) * HD + d];
                 v = fmaf(x, f[w], v);
@@ -459,8 +472,8 @@ __global__ void __launch_bounds__(kKjThreads) kv8_decode_join_kernel(const KdPar
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     pdl_wait();
     const uint32_t n = kd_span(p.a, seq).count();
-    if (n <= p.chunk) return;  // the only split wrote the output itself
-    const uint32_t used = (n + p.chunk - 1) / p.chunk;
+    const uint32_t used = kd_used(n, p.chunk);
+    if (used == 1) return;  // the only split wrote the output itself
     const uint64_t row = static_cast<uint64_t>(seq) * p.a.H + h;
     const float* ml = p.part_ml + row * p.splits * 2;
     if (warp == 0) {
@@ -503,15 +516,15 @@ __global__ void __launch_bounds__(kKjThreads) kv8_decode_join_kernel(const KdPar
 
 // ------------------------------------------------------------------- host
 
-// Pages of a split and splits of the longest sequence.  About four rounds of
-// the 2 CTAs that an SM holds, so that sequences of unlike length even out;
-// at least two pages a warp, below which starting a CTA costs more than its
+// Pages of a split and splits of the longest sequence.  About three rounds of
+// the 4 CTAs that an SM holds, so that sequences of unlike length even out;
+// at least a page a warp, below which starting a CTA costs more than its
 // pages.
 static void kd_plan(int sms, uint32_t kv, uint32_t count, uint32_t max_len, uint32_t& chunk, uint32_t& splits) {
     const uint64_t pages = (static_cast<uint64_t>(max_len) + kKv8Page - 1) / kKv8Page;
-    const uint64_t want = std::max<uint64_t>(1, 8ull * sms / (static_cast<uint64_t>(kv) * std::max(1u, count)));
+    const uint64_t want = std::max<uint64_t>(1, 12ull * sms / (static_cast<uint64_t>(kv) * std::max(1u, count)));
     const uint64_t cap = std::min<uint64_t>(want, kKdMaxSplits);
-    uint64_t c = std::max<uint64_t>((pages + cap - 1) / cap, 2 * kKdWarps);
+    uint64_t c = std::max<uint64_t>((pages + cap - 1) / cap, kKdWarps);
     c = (c + kKdWarps - 1) / kKdWarps * kKdWarps;
     chunk = static_cast<uint32_t>(c);
     splits = static_cast<uint32_t>((pages + c - 1) / c);
@@ -526,7 +539,7 @@ uint64_t kv8_decode_workspace(int sms, uint32_t hd, uint32_t kv, uint32_t heads,
 template <typename T, int HD, int TERMS, int SETS>
 static cudaError_t kd_launch(const KdParams& p, cudaStream_t s) {
     using Shape = KdShape<HD>;
-    constexpr uint32_t smem = kKdWarps * kKdRing + SETS * Shape::kSteps * 32 * 8 + kKdWarps * Shape::kItems * 8 + 8 * 4;
+    constexpr uint32_t smem = Shape::kRing + SETS * Shape::kSteps * 32 * 8 + kKdWarps * Shape::kItems * 8 + 8 * 4;
     static std::mutex mu;
     static uint64_t done = 0;
     int dev = 0;
