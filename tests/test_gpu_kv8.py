@@ -390,6 +390,28 @@ def test_masked_non_finite(ctx, dtype):
     near(out, ro, to, "prefill")
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_non_finite_in_sight(ctx, dtype, which):
+    """One page and head with a NaN: the rows and heads that see the page give NaN, all others do not."""
+    c = Cache(ctx, (4, 2, 64), dtype, [200])
+    g = torch.Generator("cuda").manual_seed(9)
+    k, v = c.random(200, g), c.random(200, g)
+    (k if which == "k" else v)[100, 1, 5] = math.nan  # page 3, KV head 1: query heads 2 and 3
+    c.append([(k, v)])
+    q = c.queries(1, g)
+    out, _ = c.decode(q)
+    assert torch.isfinite(out[0, :2]).all() and torch.isnan(out[0, 2:]).all()
+    q = c.queries(200, g)
+    for window in (0, 20):
+        out, _ = c.prefill(q, [200], window=window)
+        sees = torch.arange(200) >= 96
+        if window:
+            sees &= torch.arange(200) <= 127 + window - 1
+        assert torch.equal(torch.isnan(out).all(2).cpu(), sees[:, None] & torch.tensor([False, False, True, True]))
+        assert torch.equal(torch.isnan(out).any(2).cpu(), sees[:, None] & torch.tensor([False, False, True, True]))
+
+
 def test_out_of_range(ctx):
     """A page outside the pool is left out, a length beyond the table or max_len is cut, and the status says so."""
     c = Cache(ctx, (8, 2, 64), "f32", [128, 128, 128])

@@ -1,8 +1,9 @@
 // Paged 8-bit KV cache: the kernels that write and read its pages, and the C
-// entry points (vrt_kv8_*).  Its attention kernels are in kv8_attention.cu.
+// entry points (vrt_kv8_*).  Its attention kernels are in kv8_decode.cu and kv8_prefill.cu.
 
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "kv8.cuh"
@@ -350,15 +351,13 @@ int attention(vrt_ctx* ctx, const vrt_kv8_cache* cache, const vrt_kv8_attn* attn
     p.window = attn->window;
     p.scale = attn->scale;
     p.softcap = attn->softcap;
+    p.dtype = cache->dtype;
     p.status = status_word(ctx);
     DeviceScope dev(ctx->device);
     VRT_CUDA(dev.e);
     const int sms = ctx->prop.multiProcessorCount;
-    if (d_cu) {
-        VRT_CUDA(kv8_attention(p, cache->head_dim, cache->dtype, as_stream(ctx, stream)));
-    } else {
-        VRT_CUDA(kv8_decode(p, cache->head_dim, cache->dtype, sms, d_workspace, as_stream(ctx, stream)));
-    }
+    const auto run = d_cu ? kv8_prefill : kv8_decode;
+    VRT_CUDA(run(p, cache->head_dim, sms, d_workspace, as_stream(ctx, stream)));
     return VRT_OK;
 }
 
@@ -430,7 +429,11 @@ int vrt_kv8_workspace(vrt_ctx* ctx, const vrt_kv8_cache* cache, uint32_t heads, 
     VRT_TRY(check_heads(cache, heads));
     if (!ctx) return fail(VRT_E_INVALID, "kv8: null context");
     const int sms = ctx->prop.multiProcessorCount;
-    *bytes = kv8_decode_workspace(sms, cache->head_dim, cache->kv_heads, heads, count, max_len);
+    // of a single row each, either kernel may be meant
+    *bytes = kv8_prefill_workspace(sms, cache->head_dim, cache->kv_heads, heads, count, max_new, max_len);
+    if (max_new == 1) {
+        *bytes = std::max(*bytes, kv8_decode_workspace(sms, cache->head_dim, cache->kv_heads, heads, count, max_len));
+    }
     return VRT_OK;
 }
 

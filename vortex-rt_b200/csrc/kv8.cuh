@@ -61,7 +61,19 @@ struct Kv8Attn {
     const int32_t* prefix;
     uint32_t H, count, max_new, max_len, window;
     float scale, softcap;
+    int dtype;
     uint32_t* status;
+};
+
+// The visible pages of a row split over `splits` CTAs, whose outputs a second
+// kernel joins (kv8_join).
+struct Kv8Split {
+    Kv8Attn a;
+    uint32_t tile;    // query tokens that see their pages together
+    uint32_t chunk;   // pages of one split at most
+    uint32_t splits;  // of the longest sequence
+    float* part;      // [count][max_new][H][splits][head_dim] unnormalised outputs
+    float* part_ml;   // [count][max_new][H][splits][2] maximum (base 2) and sum
 };
 
 // Pool index of page `page` of sequence `seq`, -1 (and the status bit) when
@@ -112,14 +124,119 @@ __device__ __forceinline__ void load_row(const T* p, float (&x)[N]) {
     }
 }
 
+// The largest magnitude of a row piece, NaN ignored.
+template <int N>
+__device__ __forceinline__ float max_abs(const float (&x)[N]) {
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = fmaxf(m, fabsf(x[i]));
+    return m;
+}
+
 // The smallest key a query of position `pos` may see through the window.
 __host__ __device__ inline int64_t kv8_window_lo(int64_t pos, uint32_t window) {
     return window && pos + 1 > static_cast<int64_t>(window) ? pos + 1 - window : 0;
 }
 
+// Pages that the queries i0 .. i1 (of the call's n rows of a sequence) see:
+// [0, a) and [b0, b1).  lo: first key in the window of query i0.
+struct Kv8Span {
+    int64_t len, lo, prefix;
+    uint32_t a, b0, b1;
+    __device__ __forceinline__ uint32_t count() const { return a + b1 - b0; }
+    __device__ __forceinline__ uint32_t page(uint32_t i) const { return i < a ? i : b0 + i - a; }
+};
+
+__device__ __forceinline__ Kv8Span kv8_span(const Kv8Attn& p, uint32_t seq, uint32_t n, uint32_t i0, uint32_t i1) {
+    Kv8Span s;
+    const int64_t limit = min(static_cast<int64_t>(p.max_len), static_cast<int64_t>(p.c.pps) * kKv8Page);
+    const int64_t len = p.len[seq];
+    if (len < 0 || len > limit) atomicOr(p.status, kStatusKv8Range);
+    s.len = max(static_cast<int64_t>(0), min(len, limit));
+    s.lo = kv8_window_lo(s.len - n + i0, p.window);
+    s.prefix = p.prefix ? max(static_cast<int64_t>(0), min(static_cast<int64_t>(p.prefix[seq]), s.len)) : 0;
+    const int64_t end = max(static_cast<int64_t>(0), s.len - n + i1 + 1);
+    s.a = static_cast<uint32_t>((s.prefix + kKv8Page - 1) / kKv8Page);
+    s.b1 = max(s.a, static_cast<uint32_t>((end + kKv8Page - 1) / kKv8Page));
+    s.b0 = min(s.b1, max(s.a, static_cast<uint32_t>(s.lo / kKv8Page)));
+    return s;
+}
+
+// The splits that n visible pages use (none longer than `chunk`) and the
+// pages of each: even shares.
+__device__ __forceinline__ uint32_t kv8_used(uint32_t n, uint32_t chunk) { return n ? (n + chunk - 1) / chunk : 1u; }
+__device__ __forceinline__ uint32_t kv8_share(uint32_t n, uint32_t used) { return (n + used - 1) / used; }
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kKv8Lift = 14.0f;  // weights are held times 2^14
+
+// ln of a sum l of weights 2^(z - m): nothing seen -> -inf, NaN stays.
+__device__ __forceinline__ float kv8_lse(float m, float l) {
+    return l == 0.0f ? -INFINITY : (m == -INFINITY ? l : m / kLog2e + logf(l));
+}
+
+// What a query row is multiplied by, so that its largest magnitude m comes to
+// [2^14, 2^15): a power of two among the normal numbers, 1 for 0, infinity and NaN.
+__device__ __forceinline__ float kv8_row_unit(float m) {
+    const int ex = static_cast<int>(__float_as_uint(m) >> 23);
+    const int up = m > 0.0f && ex < 255 ? max(-126, min(126, 14 - (ex - 127))) : 0;
+    return __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b.x), "r"(b.y));
+}
+
+__device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+// Codes 0, 1 (lo) or 2, 3 (hi) of a word whose bytes were offset by 128, as
+// two fp16: the byte under the exponent of 1024, less 1024 + 128.
+__device__ __forceinline__ uint32_t codes_lo(uint32_t w) {
+    const uint32_t b = __byte_perm(w, 0x64646464u, 0x4140u);
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&b), __float2half2_rn(1152.0f));
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
+    const uint32_t b = __byte_perm(w, 0x64646464u, 0x4342u);
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&b), __float2half2_rn(1152.0f));
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ uint32_t pack_half(__half a, __half b) {
+    return static_cast<uint32_t>(__half_as_ushort(a)) | static_cast<uint32_t>(__half_as_ushort(b)) << 16;
+}
+
+// softcap * tanh(x / softcap), in base-2 units.  f32 rows take tanhf; for 16-bit
+// rows 1 - 2 / (1 + e^2y) is off by some 2^-22 of the cap, far below a weight's rounding.
+template <bool EXACT>
+__device__ __forceinline__ float capped(float x, float cap, float inv_cap) {
+    if (EXACT) return cap * tanhf(x * inv_cap) * kLog2e;
+    const float e = ex2(x * inv_cap * (2.0f * kLog2e));
+    return cap * kLog2e * (1.0f - __fdividef(2.0f, e + 1.0f));
+}
+
+// Splits of one (sequence, head) at most: the joining kernel's weights.
+constexpr uint32_t kKv8MaxSplits = 128;
+
 cudaError_t kv8_append(const Kv8Append& p, uint32_t hd, int dtype, uint32_t count, cudaStream_t s);
-cudaError_t kv8_attention(const Kv8Attn& p, uint32_t hd, int dtype, cudaStream_t s);
-cudaError_t kv8_decode(const Kv8Attn& p, uint32_t hd, int dtype, int sms, void* workspace, cudaStream_t s);
+cudaError_t kv8_join(const Kv8Split& p, uint32_t hd, int dtype, cudaStream_t s);
+cudaError_t kv8_decode(const Kv8Attn& p, uint32_t hd, int sms, void* workspace, cudaStream_t s);
+cudaError_t kv8_prefill(const Kv8Attn& p, uint32_t hd, int sms, void* workspace, cudaStream_t s);
+uint64_t kv8_prefill_workspace(int sms, uint32_t hd, uint32_t kv, uint32_t heads, uint32_t count, uint32_t max_new,
+                               uint32_t max_len);
 uint64_t kv8_decode_workspace(int sms, uint32_t hd, uint32_t kv, uint32_t heads, uint32_t count, uint32_t max_len);
 
 }  // namespace vrt

@@ -42,9 +42,6 @@ namespace vrt {
 
 constexpr int kKdWarps = 4;
 constexpr int kKdThreads = kKdWarps * 32;
-constexpr uint32_t kKdMaxSplits = 128;
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kKdLift = 14.0f;  // weights are held times 2^14
 
 template <int HD>
 struct KdShape {
@@ -61,90 +58,10 @@ struct KdShape {
     static constexpr int kSteps = HD / 16;             // k-steps of the scores, row tiles of the output
 };
 
-struct KdParams {
-    Kv8Attn a;
-    uint32_t chunk;   // pages of one split, a multiple of the warps
-    uint32_t splits;  // grid.x
-    float* part;      // [count][H][splits][head_dim] unnormalised outputs
-    float* part_ml;   // [count][H][splits][2] maximum (base 2) and sum
-};
-
-// Visible pages of one sequence's newest token: [0, a) and [b0, b1).
-struct KdSpan {
-    int64_t len, lo, prefix;
-    uint32_t a, b0, b1;
-    __device__ __forceinline__ uint32_t count() const { return a + b1 - b0; }
-    __device__ __forceinline__ uint32_t page(uint32_t i) const { return i < a ? i : b0 + i - a; }
-};
-
-// The splits that a sequence of n visible pages uses (none longer than
-// `chunk`) and the pages of each: even shares.
-__device__ __forceinline__ uint32_t kd_used(uint32_t n, uint32_t chunk) { return n ? (n + chunk - 1) / chunk : 1u; }
-__device__ __forceinline__ uint32_t kd_share(uint32_t n, uint32_t used) { return (n + used - 1) / used; }
-
-__device__ __forceinline__ KdSpan kd_span(const Kv8Attn& p, uint32_t seq) {
-    KdSpan s;
-    const int64_t limit = min(static_cast<int64_t>(p.max_len), static_cast<int64_t>(p.c.pps) * kKv8Page);
-    const int64_t len = p.len[seq];
-    if (len < 0 || len > limit) atomicOr(p.status, kStatusKv8Range);
-    s.len = max(static_cast<int64_t>(0), min(len, limit));
-    s.lo = kv8_window_lo(s.len - 1, p.window);
-    s.prefix = p.prefix ? max(static_cast<int64_t>(0), min(static_cast<int64_t>(p.prefix[seq]), s.len)) : 0;
-    s.a = static_cast<uint32_t>((s.prefix + kKv8Page - 1) / kKv8Page);
-    s.b1 = static_cast<uint32_t>((s.len + kKv8Page - 1) / kKv8Page);
-    s.b0 = min(s.b1, max(s.a, static_cast<uint32_t>(s.lo / kKv8Page)));
-    return s;
-}
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b.x), "r"(b.y));
-}
-
-__device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
-    uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-    return y;
-}
-
-// Codes 0, 1 (lo) or 2, 3 (hi) of a word whose bytes were offset by 128, as
-// two fp16: the byte under the exponent of 1024, less 1024 + 128.
-__device__ __forceinline__ uint32_t codes_lo(uint32_t w) {
-    const uint32_t b = __byte_perm(w, 0x64646464u, 0x4140u);
-    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&b), __float2half2_rn(1152.0f));
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
-    const uint32_t b = __byte_perm(w, 0x64646464u, 0x4342u);
-    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&b), __float2half2_rn(1152.0f));
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-__device__ __forceinline__ uint32_t pack_half(__half a, __half b) {
-    return static_cast<uint32_t>(__half_as_ushort(a)) | static_cast<uint32_t>(__half_as_ushort(b)) << 16;
-}
-
-// softcap * tanh(x / softcap), in base-2 units.  f32 rows take tanhf; for 16-bit
-// rows 1 - 2 / (1 + e^2y) is off by some 2^-22 of the cap, far below a weight's rounding.
-template <bool EXACT>
-__device__ __forceinline__ float capped(float x, float cap, float inv_cap) {
-    if (EXACT) return cap * tanhf(x * inv_cap) * kLog2e;
-    const float e = ex2(x * inv_cap * (2.0f * kLog2e));
-    return cap * kLog2e * (1.0f - __fdividef(2.0f, e + 1.0f));
-}
-
 // TERMS: fp16 terms of an operand (2 for f32 rows).  SETS: mma of each step
 // (2: more than 4 heads with remainders).
 template <typename T, int HD, int TERMS, int SETS>
-__global__ void __launch_bounds__(kKdThreads, KdShape<HD>::kCtas) kv8_decode_kernel(const KdParams p) {
+__global__ void __launch_bounds__(kKdThreads, KdShape<HD>::kCtas) kv8_decode_kernel(const Kv8Split p) {
     using Shape = KdShape<HD>;
     constexpr bool kPacked = TERMS == 2 && SETS == 1;  // columns 4..7 are the remainders of heads 0..3
     constexpr int D = Shape::kItems, KS = Shape::kSteps, W = kKdWarps;
@@ -157,8 +74,8 @@ __global__ void __launch_bounds__(kKdThreads, KdShape<HD>::kCtas) kv8_decode_ker
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t4 = lane & 3;
     const uint32_t split = blockIdx.x, g = blockIdx.y, seq = blockIdx.z, R = p.a.H / p.a.c.kv;
     pdl_trigger();
-    const KdSpan span = kd_span(p.a, seq);
-    const uint32_t n = span.count(), used_splits = kd_used(n, p.chunk), share = kd_share(n, used_splits);
+    const Kv8Span span = kv8_span(p.a, seq, 1, 0, 0);
+    const uint32_t n = span.count(), used_splits = kv8_used(n, p.chunk), share = kv8_share(n, used_splits);
     if (split >= used_splits) return;
     const uint32_t j0 = min(n, split * share), j1 = min(n, j0 + share);
 
@@ -214,10 +131,7 @@ __global__ void __launch_bounds__(kKdThreads, KdShape<HD>::kCtas) kv8_decode_ker
         }
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        // 2^(14 - exponent of the largest), within the normal numbers
-        const int ex = static_cast<int>(__float_as_uint(m) >> 23);
-        const int up = m > 0.0f && ex < 255 ? max(-126, min(126, 14 - (ex - 127))) : 0;
-        const float mul = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
+        const float mul = kv8_row_unit(m);
         if (piece == 0) q_unit[h] = 1.0f / mul;
         __half* f = reinterpret_cast<__half*>(qf);
 #pragma unroll
@@ -346,7 +260,7 @@ __global__ void __launch_bounds__(kKdThreads, KdShape<HD>::kCtas) kv8_decode_ker
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[q][e] *= f[e & 1];
         }
-        const float m0[2] = {mx[0] == -INFINITY ? 0.0f : mx[0] - kKdLift, mx[1] == -INFINITY ? 0.0f : mx[1] - kKdLift};
+        const float m0[2] = {mx[0] == -INFINITY ? 0.0f : mx[0] - kKv8Lift, mx[1] == -INFINITY ? 0.0f : mx[1] - kKv8Lift};
         uint32_t ph[4], pl[4];
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
@@ -413,7 +327,7 @@ __global__ void __launch_bounds__(kKdThreads, KdShape<HD>::kCtas) kv8_decode_ker
     if (g8 == 0 && (!kPacked || t4 < 2)) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            wm[(warp * 8 + 2 * t4 + h) * 2] = mx[h] - kKdLift;  // sums are times 2^14
+            wm[(warp * 8 + 2 * t4 + h) * 2] = mx[h] - kKv8Lift;  // sums are times 2^14
             wm[(warp * 8 + 2 * t4 + h) * 2 + 1] = sum[h];
         }
     }
@@ -449,68 +363,12 @@ __global__ void __launch_bounds__(kKdThreads, KdShape<HD>::kCtas) kv8_decode_ker
         }
         if (lane == 0) {
             if (alone) {
-                if (p.a.lse) p.a.lse[row] = l == 0.0f ? -INFINITY : (m == -INFINITY ? l : m / kLog2e + logf(l));
+                if (p.a.lse) p.a.lse[row] = kv8_lse(m, l);
             } else {
                 p.part_ml[(row * p.splits + split) * 2] = m;
                 p.part_ml[(row * p.splits + split) * 2 + 1] = l;
             }
         }
-    }
-}
-
-constexpr int kKjThreads = 256;
-
-// CTA (head, sequence): the splits' outputs in split order, 8 warps over the
-// splits, then over each other.
-template <typename T, int HD>
-__global__ void __launch_bounds__(kKjThreads) kv8_decode_join_kernel(const KdParams p) {
-    constexpr int W = kKjThreads / 32;
-    __shared__ float f[kKdMaxSplits];
-    __shared__ float o[W][HD];
-    __shared__ float total;
-    const uint32_t h = blockIdx.x, seq = blockIdx.y;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    pdl_wait();
-    const uint32_t n = kd_span(p.a, seq).count();
-    const uint32_t used = kd_used(n, p.chunk);
-    if (used == 1) return;  // the only split wrote the output itself
-    const uint64_t row = static_cast<uint64_t>(seq) * p.a.H + h;
-    const float* ml = p.part_ml + row * p.splits * 2;
-    if (warp == 0) {
-        float m = -INFINITY, l = 0.0f;
-        for (uint32_t i = lane; i < used; i += 32) m = fmaxf(m, ml[2 * i]);
-#pragma unroll
-        for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-        for (uint32_t i = lane; i < used; i += 32) {
-            f[i] = ml[2 * i] == -INFINITY ? 1.0f : ex2(ml[2 * i] - m);
-            l += ml[2 * i + 1] * f[i];
-        }
-        l = warp_sum(l);
-        if (lane == 0) {
-            total = l;
-            if (p.a.lse) p.a.lse[row] = l == 0.0f ? -INFINITY : (m == -INFINITY ? l : m / kLog2e + logf(l));
-        }
-    }
-    __syncthreads();
-    const float* part = p.part + row * p.splits * HD;
-    float v[HD / 32];
-#pragma unroll
-    for (int e = 0; e < HD / 32; ++e) v[e] = 0.0f;
-#pragma unroll 4
-    for (uint32_t i = warp; i < used; i += W) {
-#pragma unroll
-        for (int e = 0; e < HD / 32; ++e) v[e] = fmaf(part[static_cast<uint64_t>(i) * HD + lane + 32 * e], f[i], v[e]);
-    }
-#pragma unroll
-    for (int e = 0; e < HD / 32; ++e) o[warp][lane + 32 * e] = v[e];
-    __syncthreads();
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    T* out = static_cast<T*>(p.a.out) + static_cast<uint64_t>(seq) * p.a.out_stride + static_cast<uint64_t>(h) * HD;
-    for (int d = threadIdx.x; d < HD; d += kKjThreads) {
-        float x = 0.0f;
-#pragma unroll
-        for (int w = 0; w < W; ++w) x += o[w][d];
-        out[d] = from_f32<T>(x * inv);
     }
 }
 
@@ -523,7 +381,7 @@ __global__ void __launch_bounds__(kKjThreads) kv8_decode_join_kernel(const KdPar
 static void kd_plan(int sms, uint32_t kv, uint32_t count, uint32_t max_len, uint32_t& chunk, uint32_t& splits) {
     const uint64_t pages = (static_cast<uint64_t>(max_len) + kKv8Page - 1) / kKv8Page;
     const uint64_t want = std::max<uint64_t>(1, 12ull * sms / (static_cast<uint64_t>(kv) * std::max(1u, count)));
-    const uint64_t cap = std::min<uint64_t>(want, kKdMaxSplits);
+    const uint64_t cap = std::min<uint64_t>(want, kKv8MaxSplits);
     uint64_t c = std::max<uint64_t>((pages + cap - 1) / cap, kKdWarps);
     c = (c + kKdWarps - 1) / kKdWarps * kKdWarps;
     chunk = static_cast<uint32_t>(c);
@@ -537,7 +395,7 @@ uint64_t kv8_decode_workspace(int sms, uint32_t hd, uint32_t kv, uint32_t heads,
 }
 
 template <typename T, int HD, int TERMS, int SETS>
-static cudaError_t kd_launch(const KdParams& p, cudaStream_t s) {
+static cudaError_t kd_launch(const Kv8Split& p, cudaStream_t s) {
     using Shape = KdShape<HD>;
     constexpr uint32_t smem = Shape::kRing + SETS * Shape::kSteps * 32 * 8 + kKdWarps * Shape::kItems * 8 + 8 * 4;
     static std::mutex mu;
@@ -556,12 +414,14 @@ static cudaError_t kd_launch(const KdParams& p, cudaStream_t s) {
     }
     e = launch(kv8_decode_kernel<T, HD, TERMS, SETS>, dim3(p.splits, p.a.c.kv, p.a.count), dim3(kKdThreads), smem, s, false, p);
     if (e != cudaSuccess || p.splits == 1) return e;
-    return launch(kv8_decode_join_kernel<T, HD>, dim3(p.a.H, p.a.count), dim3(kKjThreads), 0, s, true, p);
+    return kv8_join(p, HD, p.a.dtype, s);
 }
 
-cudaError_t kv8_decode(const Kv8Attn& a, uint32_t hd, int dtype, int sms, void* workspace, cudaStream_t s) {
-    KdParams p{};
+cudaError_t kv8_decode(const Kv8Attn& a, uint32_t hd, int sms, void* workspace, cudaStream_t s) {
+    Kv8Split p{};
     p.a = a;
+    p.tile = 1;
+    const int dtype = a.dtype;
     kd_plan(sms, a.c.kv, a.count, a.max_len, p.chunk, p.splits);
     p.part = static_cast<float*>(workspace);
     p.part_ml = p.part + static_cast<uint64_t>(a.count) * a.H * p.splits * hd;
