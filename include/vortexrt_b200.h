@@ -446,6 +446,13 @@ typedef struct vrt_batch vrt_batch;
  * GEMMs used instead, when it does not fit). */
 VRT_API int vrt_batch_create(vrt_model* m, uint32_t max_seqs, uint32_t max_positions, int keep_logits,
                              vrt_batch** out);
+/* The same with keys and values held in 8 bits (the paged cache above, fp32
+ * rows): a quarter of the cache's bytes, on sliding layers a ring of the
+ * window and 512 more tokens.  A value is off by at most 1/254 of the largest
+ * of its page and head, so results are those of a slightly rounded cache, not
+ * the fp32 cache's. */
+VRT_API int vrt_batch_create_kv8(vrt_model* m, uint32_t max_seqs, uint32_t max_positions, int keep_logits,
+                                 vrt_batch** out);
 VRT_API int vrt_batch_destroy(vrt_batch* b);
 /* Prefill sequence `seq` (batched tensor-core prefill into its cache); emits its
  * first greedy id and sets its position to n. */

@@ -34,6 +34,7 @@
 
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <mutex>
 
 #include "kv8.cuh"
@@ -374,23 +375,28 @@ __global__ void __launch_bounds__(kKdThreads, KdShape<HD>::kCtas) kv8_decode_ker
 
 // ------------------------------------------------------------------- host
 
-// Pages of a split and splits of the longest sequence.  About three rounds of
+static uint64_t kd_cap(int sms, uint32_t kv, uint32_t count) {
+    const uint64_t want = 12ull * sms / (static_cast<uint64_t>(kv) * std::max(1u, count));
+    return std::min<uint64_t>(std::max<uint64_t>(1, want), kKv8MaxSplits);
+}
+
+// Pages of a split and splits of a sequence that sees `pages` pages.  About three rounds of
 // the 4 CTAs that an SM holds, so that sequences of unlike length even out;
 // at least a page a warp, below which starting a CTA costs more than its
 // pages.
-static void kd_plan(int sms, uint32_t kv, uint32_t count, uint32_t max_len, uint32_t& chunk, uint32_t& splits) {
-    const uint64_t pages = (static_cast<uint64_t>(max_len) + kKv8Page - 1) / kKv8Page;
-    const uint64_t want = std::max<uint64_t>(1, 12ull * sms / (static_cast<uint64_t>(kv) * std::max(1u, count)));
-    const uint64_t cap = std::min<uint64_t>(want, kKv8MaxSplits);
+static void kd_plan(int sms, uint32_t kv, uint32_t count, uint64_t pages, uint32_t& chunk, uint32_t& splits) {
+    const uint64_t cap = kd_cap(sms, kv, count);
     uint64_t c = std::max<uint64_t>((pages + cap - 1) / cap, kKdWarps);
     c = (c + kKdWarps - 1) / kKdWarps * kKdWarps;
     chunk = static_cast<uint32_t>(c);
     splits = static_cast<uint32_t>((pages + c - 1) / c);
 }
 
+// For any number of visible pages up to max_len's: no plan has more splits
+// than its cap, nor than one for each kKdWarps pages.
 uint64_t kv8_decode_workspace(int sms, uint32_t hd, uint32_t kv, uint32_t heads, uint32_t count, uint32_t max_len) {
-    uint32_t chunk, splits;
-    kd_plan(sms, kv, count, max_len, chunk, splits);
+    const uint64_t pages = (static_cast<uint64_t>(max_len) + kKv8Page - 1) / kKv8Page;
+    const uint64_t splits = std::min<uint64_t>(kd_cap(sms, kv, count), (pages + kKdWarps - 1) / kKdWarps);
     return splits > 1 ? static_cast<uint64_t>(count) * heads * splits * (hd + 2) * 4 : 0;
 }
 
@@ -422,7 +428,10 @@ cudaError_t kv8_decode(const Kv8Attn& a, uint32_t hd, int sms, void* workspace, 
     p.a = a;
     p.tile = 1;
     const int dtype = a.dtype;
-    kd_plan(sms, a.c.kv, a.count, a.max_len, p.chunk, p.splits);
+    uint64_t pages = (static_cast<uint64_t>(a.max_len) + kKv8Page - 1) / kKv8Page;
+    // a window's tokens lie in one page more than they fill; a prefix adds its own
+    if (a.window && !a.prefix) pages = std::min<uint64_t>(pages, (static_cast<uint64_t>(a.window) + kKv8Page - 2) / kKv8Page + 1);
+    kd_plan(sms, a.c.kv, a.count, pages, p.chunk, p.splits);
     p.part = static_cast<float*>(workspace);
     p.part_ml = p.part + static_cast<uint64_t>(a.count) * a.H * p.splits * hd;
     const bool wide = a.H / a.c.kv > 4;

@@ -374,28 +374,30 @@ cudaError_t kv8_join(const Kv8Split& p, uint32_t hd, int dtype, cudaStream_t s) 
 }
 
 // Splits of a history when there are too few query tiles for the GPU: about
-// two CTAs an SM, 8 pages each at least.
-static void kp_plan(int sms, uint32_t kv, uint32_t heads, uint32_t count, uint32_t max_new, uint32_t max_len,
-                    uint32_t& tile, uint32_t& chunk, uint32_t& splits) {
-    tile = kKpRows / (heads / kv);
-    const uint64_t pages = (static_cast<uint64_t>(max_len) + kKv8Page - 1) / kKv8Page;
+// two CTAs an SM, kKpMinPages pages each at least.
+constexpr uint32_t kKpMinPages = 8;
+
+static uint64_t kp_cap(int sms, uint32_t tile, uint32_t kv, uint32_t count, uint32_t max_new) {
     const uint64_t ctas = (static_cast<uint64_t>(max_new) + tile - 1) / tile * kv * std::max(1u, count);
-    uint64_t want = std::min<uint64_t>(2ull * sms / std::max<uint64_t>(1, ctas), kKv8MaxSplits);
-    want = std::min<uint64_t>(want, 65535u / std::max(1u, count));  // grid.z
-    if (want <= 1 || max_new > 65535u) {
-        chunk = static_cast<uint32_t>(pages);
-        splits = 1;
-        return;
-    }
-    const uint64_t c = std::max<uint64_t>((pages + want - 1) / want, 8);
+    const uint64_t want = std::min<uint64_t>(2ull * sms / std::max<uint64_t>(1, ctas), kKv8MaxSplits);
+    return max_new > 65535u ? 1 : std::max<uint64_t>(1, std::min<uint64_t>(want, 65535u / std::max(1u, count)));  // grid limits
+}
+
+static void kp_plan(int sms, const Kv8Attn& a, uint32_t& tile, uint32_t& chunk, uint32_t& splits) {
+    tile = kKpRows / (a.H / a.c.kv);
+    const uint64_t pages = (static_cast<uint64_t>(a.max_len) + kKv8Page - 1) / kKv8Page;
+    const uint64_t cap = kp_cap(sms, tile, a.c.kv, a.count, a.max_new);
+    const uint64_t c = std::max<uint64_t>((pages + cap - 1) / cap, kKpMinPages);
     chunk = static_cast<uint32_t>(c);
     splits = static_cast<uint32_t>((pages + c - 1) / c);
 }
 
+// For any max_len up to this one, as in kv8_decode_workspace.
 uint64_t kv8_prefill_workspace(int sms, uint32_t hd, uint32_t kv, uint32_t heads, uint32_t count, uint32_t max_new,
                                uint32_t max_len) {
-    uint32_t tile, chunk, splits;
-    kp_plan(sms, kv, heads, count, max_new, max_len, tile, chunk, splits);
+    const uint64_t pages = (static_cast<uint64_t>(max_len) + kKv8Page - 1) / kKv8Page;
+    const uint64_t splits = std::min<uint64_t>(kp_cap(sms, kKpRows / (heads / kv), kv, count, max_new),
+                                               (pages + kKpMinPages - 1) / kKpMinPages);
     return splits > 1 ? static_cast<uint64_t>(count) * max_new * heads * splits * (hd + 2) * 4 : 0;
 }
 
@@ -425,7 +427,7 @@ static cudaError_t kp_launch(const Kv8Split& p, cudaStream_t s) {
 cudaError_t kv8_prefill(const Kv8Attn& a, uint32_t hd, int sms, void* workspace, cudaStream_t s) {
     Kv8Split p{};
     p.a = a;
-    kp_plan(sms, a.c.kv, a.H, a.count, a.max_new, a.max_len, p.tile, p.chunk, p.splits);
+    kp_plan(sms, a, p.tile, p.chunk, p.splits);
     p.part = static_cast<float*>(workspace);
     p.part_ml = p.part + static_cast<uint64_t>(a.count) * a.max_new * a.H * p.splits * hd;
 #define VRT_KP(HD)                                                                \

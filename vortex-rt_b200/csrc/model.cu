@@ -42,6 +42,7 @@
 #include "vortexrt/gguf.hpp"
 #include "vrt_device.cuh"
 #include "vrt_internal.hpp"
+#include "kv8.cuh"
 #include "vrt_kernels.hpp"
 
 namespace vrt {
@@ -354,6 +355,15 @@ struct vrt_batch {
     int8_t *q_hi = nullptr, *q_lo = nullptr;
     float *q_sx = nullptr, *att32 = nullptr, *act32 = nullptr;
     vrt::TmaMap Qd_hi, Qd_lo, Qq_hi, Qq_lo, Qf_hi, Qf_lo;
+    // 8-bit KV cache (vrt_batch_create_kv8): per layer the pages of all
+    // sequences; a global layer's table is linear, a sliding layer's pages of
+    // one sequence are a ring of the window and one prefill slice
+    bool kv8 = false;
+    std::vector<vrt::Kv8View> kv8_layer;
+    int32_t* kv8_len = nullptr;                // [S] tokens held, this step's included
+    int32_t* kv8_meta = nullptr;               // start, cu[2], len of the prefill slice at hand
+    float *kv8_q = nullptr, *kv8_k = nullptr, *kv8_v = nullptr;  // [S][heads][hd] this step's rows
+    void* kv8_ws = nullptr;
 };
 
 namespace vrt {
@@ -1485,16 +1495,19 @@ static cudaError_t prefill_attn_launch(const PrefillAttnParams& a, uint32_t hd, 
     }
 }
 
+// Rows at positions p0 + row, or at pos[row] (device) when pos is given;
+// len[row] then receives that position + 1.
 static cudaError_t qk_rope_launch(const float* qkv, vrt_model* m, const LayerW& L, uint32_t p0, uint32_t n, float* q,
-                                  float* k, float* v, cudaStream_t s) {
+                                  float* k, float* v, cudaStream_t s, const uint32_t* pos = nullptr,
+                                  int32_t* len = nullptr) {
     const auto& c = m->cfg;
     auto F = [&](uint64_t off) { return reinterpret_cast<const float*>(m->arena + off); };
     const float* cs = L.global ? m->rope_cos_g : m->rope_cos_l;
     const float* sn = L.global ? m->rope_sin_g : m->rope_sin_l;
     switch (c.head_dim) {
-    case 64: qk_rope_rows_kernel<2><<<n, 256, 0, s>>>(qkv, m->Hl, m->KVl, F(L.n_q), F(L.n_k), cs, sn, p0, c.rms_epsilon, q, k, v); break;
-    case 128: qk_rope_rows_kernel<4><<<n, 256, 0, s>>>(qkv, m->Hl, m->KVl, F(L.n_q), F(L.n_k), cs, sn, p0, c.rms_epsilon, q, k, v); break;
-    case 256: qk_rope_rows_kernel<8><<<n, 256, 0, s>>>(qkv, m->Hl, m->KVl, F(L.n_q), F(L.n_k), cs, sn, p0, c.rms_epsilon, q, k, v); break;
+    case 64: qk_rope_rows_kernel<2><<<n, 256, 0, s>>>(qkv, m->Hl, m->KVl, F(L.n_q), F(L.n_k), cs, sn, p0, pos, len, c.rms_epsilon, q, k, v); break;
+    case 128: qk_rope_rows_kernel<4><<<n, 256, 0, s>>>(qkv, m->Hl, m->KVl, F(L.n_q), F(L.n_k), cs, sn, p0, pos, len, c.rms_epsilon, q, k, v); break;
+    case 256: qk_rope_rows_kernel<8><<<n, 256, 0, s>>>(qkv, m->Hl, m->KVl, F(L.n_q), F(L.n_k), cs, sn, p0, pos, len, c.rms_epsilon, q, k, v); break;
     default: return cudaErrorInvalidValue;
     }
     return cudaGetLastError();
@@ -1519,7 +1532,68 @@ struct SeqTarget {
     unsigned long long* key = nullptr;   // argmax key (zero on entry)
     float* hidden = nullptr;             // normed hidden of the last token
     float* logits = nullptr;             // optional full logits of the last token
+    const vrt_batch* kv8 = nullptr;      // 8-bit cache: sequence `seq` of this batch instead of kc, vc, cap
+    uint32_t seq = 0;
 };
+
+// Tokens that a sliding layer's 8-bit ring takes at once on top of its window.
+constexpr uint32_t kKv8Slice = 512;
+
+static Kv8Attn kv8_attn(const vrt_model* m, const Kv8View& view, bool global, uint32_t positions, const float* q, float* out) {
+    Kv8Attn a{};
+    a.c = view;
+    a.q = q;
+    a.out = out;
+    a.q_stride = a.out_stride = static_cast<uint64_t>(m->Hl) * m->cfg.head_dim;
+    a.H = m->Hl;
+    a.count = a.max_new = 1;
+    a.max_len = positions;
+    a.window = global ? 0u : m->cfg.sliding_window;
+    a.scale = 1.0f / std::sqrt(static_cast<float>(m->cfg.head_dim));
+    a.dtype = VRT_F32;
+    a.status = &m->st->status;
+    return a;
+}
+
+// Layer l's attention of the chunk's nc tokens from position p0 through the
+// 8-bit cache: slice by slice, append then attend.  Output rows -> pf.qkv,
+// then the o-projection operand.
+static int kv8_prefill_layer(vrt_model* m, const SeqTarget& t, uint32_t l, uint32_t p0, uint32_t nc, cudaStream_t s) {
+    const vrt_batch* b = t.kv8;
+    auto& B = m->pf;
+    const bool global = m->layers[l].global;
+    const uint32_t hd = m->cfg.head_dim, kvw = m->KVl * hd, qw = m->Hl * hd;
+    Kv8View view = b->kv8_layer[l];  // of this sequence alone
+    view.table += static_cast<uint64_t>(t.seq) * view.pps;
+    view.k_tail = static_cast<float*>(view.k_tail) + static_cast<uint64_t>(t.seq) * kKv8Page * kvw;
+    view.v_tail = static_cast<float*>(view.v_tail) + static_cast<uint64_t>(t.seq) * kKv8Page * kvw;
+    view.max_seqs = 1;
+    const uint32_t slice = global ? nc : std::min(nc, kKv8Slice);
+    for (uint32_t i = 0; i < nc; i += slice) {
+        const int32_t n = static_cast<int32_t>(std::min(slice, nc - i)), at = static_cast<int32_t>(p0 + i);
+        const int32_t meta[4] = {at, 0, n, at + n};
+        VRT_CUDA(cudaMemcpyAsync(b->kv8_meta, meta, sizeof meta, cudaMemcpyHostToDevice, s));
+        Kv8Append ap{};
+        ap.c = view;
+        ap.k = B.k + static_cast<uint64_t>(i) * kvw;
+        ap.v = B.v + static_cast<uint64_t>(i) * kvw;
+        ap.stride = kvw;
+        ap.start = b->kv8_meta;
+        ap.cu = b->kv8_meta + 1;
+        ap.max_new = static_cast<uint32_t>(n);
+        ap.status = &m->st->status;
+        VRT_CUDA(kv8_append(ap, hd, VRT_F32, 1, s));
+        const uint64_t row = static_cast<uint64_t>(i) * qw;
+        Kv8Attn a = kv8_attn(m, view, global, b->P, B.q + row, B.qkv + row);
+        a.len = b->kv8_meta + 3;
+        a.cu = b->kv8_meta + 1;
+        a.max_new = static_cast<uint32_t>(n);
+        a.max_len = std::min(b->P, static_cast<uint32_t>(at + n));
+        VRT_CUDA(kv8_prefill(a, hd, m->ctx->prop.multiProcessorCount, b->kv8_ws, s));
+    }
+    VRT_CUDA(split_f16(B.qkv, static_cast<uint64_t>(nc) * qw, B.xh, B.xl, s));
+    return VRT_OK;
+}
 
 static SeqTarget model_target(vrt_model* m) {
     SeqTarget t;
@@ -1581,24 +1655,28 @@ static int prefill_layers(vrt_model* m, const SeqTarget& t, uint32_t n) {
             VRT_TRY(gemm(kGemmStore, B.xd_hi, B.xd_lo, m->arena + L.qkv, m->qwl + 2 * m->kwl, d, nc, B.qkv, nullptr,
                          nullptr));
             VRT_CUDA(qk_rope_launch(B.qkv, m, L, p0, nc, B.q, B.k, B.v, s));
-            PrefillAttnParams a{};
-            a.q = B.q;
-            a.k = B.k;
-            a.v = B.v;
-            a.k_cache = t.kc[l];
-            a.v_cache = t.vc[l];
-            a.cap = t.cap[l];
-            a.window = L.global ? 0u : c.sliding_window;
-            a.p0 = p0;
-            a.n = nc;
-            a.H = m->Hl;
-            a.KV = m->KVl;
-            a.scale = 1.0f / std::sqrt(static_cast<float>(hd));
-            a.out_hi = B.xh;
-            a.out_lo = B.xl;
-            VRT_CUDA(prefill_attn_launch(a, hd, G, s));
-            kv_store_kernel<<<dim3(nc, m->KVl), 128, 0, s>>>(B.k, B.v, t.kc[l], t.vc[l], t.cap[l], m->KVl, hd, p0, nc);
-            VRT_CUDA(cudaGetLastError());
+            if (t.kv8) {
+                VRT_TRY(kv8_prefill_layer(m, t, l, p0, nc, s));
+            } else {
+                PrefillAttnParams a{};
+                a.q = B.q;
+                a.k = B.k;
+                a.v = B.v;
+                a.k_cache = t.kc[l];
+                a.v_cache = t.vc[l];
+                a.cap = t.cap[l];
+                a.window = L.global ? 0u : c.sliding_window;
+                a.p0 = p0;
+                a.n = nc;
+                a.H = m->Hl;
+                a.KV = m->KVl;
+                a.scale = 1.0f / std::sqrt(static_cast<float>(hd));
+                a.out_hi = B.xh;
+                a.out_lo = B.xl;
+                VRT_CUDA(prefill_attn_launch(a, hd, G, s));
+                kv_store_kernel<<<dim3(nc, m->KVl), 128, 0, s>>>(B.k, B.v, t.kc[l], t.vc[l], t.cap[l], m->KVl, hd, p0, nc);
+                VRT_CUDA(cudaGetLastError());
+            }
             VRT_TRY(gemm(kGemmStore, B.xq_hi, B.xq_lo, m->arena + L.o, d, m->qwl, nc, B.o, nullptr, nullptr));
             VRT_TRY(nccl_sum(m, B.o, static_cast<size_t>(nc) * d, s));  // row-parallel partials (tensor parallel)
             resid_rows_kernel<<<nc, kRowThreads, 0, s>>>(B.o, B.h0, F(L.n_post_attn), F(L.n_ffn), c.rms_epsilon, d,
@@ -1731,6 +1809,28 @@ static int batch_gemm_workspace(vrt_batch* b, uint32_t count) {
     return VRT_OK;
 }
 
+// Pages of the ring that holds a sliding layer's window and one prefill
+// slice: the window's first token and the slice's last may both lie anywhere
+// in their pages.
+static uint64_t kv8_ring_pages(uint32_t window) { return (static_cast<uint64_t>(window) + kKv8Slice + kKv8Page - 1) / kKv8Page + 1; }
+
+// Pages of one sequence in layer l's 8-bit cache.
+static uint64_t batch_kv8_pages(const vrt_model* m, uint32_t l, uint32_t positions) {
+    const uint64_t pps = (static_cast<uint64_t>(positions) + kKv8Page - 1) / kKv8Page;
+    return m->layers[l].global ? pps : std::min(pps, kv8_ring_pages(m->cfg.sliding_window));
+}
+
+// Workspace for every step and prefill slice that the batch may run.
+static uint64_t batch_kv8_workspace(const vrt_model* m, uint32_t max_seqs, uint32_t positions) {
+    const int sms = m->ctx->prop.multiProcessorCount;
+    const uint32_t hd = m->cfg.head_dim, chunk = m->opt.prefill_chunk ? m->opt.prefill_chunk : 2048u;
+    uint64_t most = 16;
+    for (uint32_t n = 1; n <= max_seqs; ++n) most = std::max(most, kv8_decode_workspace(sms, hd, m->KVl, m->Hl, n, positions));
+    for (uint32_t n = 1; n <= std::min(chunk, positions); ++n)
+        most = std::max(most, kv8_prefill_workspace(sms, hd, m->KVl, m->Hl, 1, n, positions));
+    return most;
+}
+
 // One decode step for sequences [0, count) on the model stream.
 static int batch_record_step(vrt_batch* b, uint32_t count) {
     vrt_model* m = b->m;
@@ -1814,36 +1914,54 @@ static int batch_record_step(vrt_batch* b, uint32_t count) {
         } else {
             VRT_TRY(gemm(kGemmStore, b->xd_hi, b->xd_lo, m->arena + L.qkv, qkvw, d, b->qkv, nullptr, nullptr));
         }
-        AttnParams a{};
-        a.qkv = b->qkv;
-        a.q_norm = F(L.n_q);
-        a.k_norm = F(L.n_k);
-        a.rope_cos = L.global ? m->rope_cos_g : m->rope_cos_l;
-        a.rope_sin = L.global ? m->rope_sin_g : m->rope_sin_l;
-        a.k_cache = b->kc[l];
-        a.v_cache = b->vc[l];
-        a.cap = b->cap[l];
-        a.window = L.global ? 0u : c.sliding_window;
-        a.pos = b->pos;
-        a.H = m->Hl;
-        a.KV = m->KVl;
-        a.hd = hd;
-        a.eps = c.rms_epsilon;
-        a.scale = 1.0f / std::sqrt(static_cast<float>(hd));
-        a.part_ml = b->part_ml;
-        a.part_acc = b->part_acc;
-        a.tickets = b->tickets;
-        a.splits = batch_splits(b, count, b->cap[l]);
-        a.seq_qkv = qkvw;
-        a.seq_cache = static_cast<uint64_t>(m->KVl) * b->cap[l] * hd;
-        a.seq_out = m->qwl;
-        if (i8) {
-            a.out = b->att32;
+        if (b->kv8) {
+            VRT_CUDA(qk_rope_launch(b->qkv, m, L, 0, count, b->kv8_q, b->kv8_k, b->kv8_v, s, b->pos, b->kv8_len));
+            Kv8Append ap{};
+            ap.c = b->kv8_layer[l];
+            ap.k = b->kv8_k;
+            ap.v = b->kv8_v;
+            ap.stride = static_cast<uint64_t>(m->KVl) * hd;
+            ap.start = reinterpret_cast<const int32_t*>(b->pos);
+            ap.max_new = 1;
+            ap.status = status;
+            VRT_CUDA(kv8_append(ap, hd, VRT_F32, count, s));
+            Kv8Attn a = kv8_attn(m, b->kv8_layer[l], L.global, b->P, b->kv8_q, b->att32);
+            a.len = b->kv8_len;
+            a.count = count;
+            VRT_CUDA(kv8_decode(a, hd, m->ctx->prop.multiProcessorCount, b->kv8_ws, s));
+            if (!i8) VRT_CUDA(split_f16(b->att32, static_cast<uint64_t>(count) * m->qwl, b->xh, b->xl, s));
         } else {
-            a.out_hi = b->xh;
-            a.out_lo = b->xl;
+            AttnParams a{};
+            a.qkv = b->qkv;
+            a.q_norm = F(L.n_q);
+            a.k_norm = F(L.n_k);
+            a.rope_cos = L.global ? m->rope_cos_g : m->rope_cos_l;
+            a.rope_sin = L.global ? m->rope_sin_g : m->rope_sin_l;
+            a.k_cache = b->kc[l];
+            a.v_cache = b->vc[l];
+            a.cap = b->cap[l];
+            a.window = L.global ? 0u : c.sliding_window;
+            a.pos = b->pos;
+            a.H = m->Hl;
+            a.KV = m->KVl;
+            a.hd = hd;
+            a.eps = c.rms_epsilon;
+            a.scale = 1.0f / std::sqrt(static_cast<float>(hd));
+            a.part_ml = b->part_ml;
+            a.part_acc = b->part_acc;
+            a.tickets = b->tickets;
+            a.splits = batch_splits(b, count, b->cap[l]);
+            a.seq_qkv = qkvw;
+            a.seq_cache = static_cast<uint64_t>(m->KVl) * b->cap[l] * hd;
+            a.seq_out = m->qwl;
+            if (i8) {
+                a.out = b->att32;
+            } else {
+                a.out_hi = b->xh;
+                a.out_lo = b->xl;
+            }
+            VRT_CUDA(attention_launch(a, dim3(a.splits, m->KVl, count), s, false));
         }
-        VRT_CUDA(attention_launch(a, dim3(a.splits, m->KVl, count), s, false));
         if (i8) {
             VRT_CUDA(quant_rows(b->att32, m->qwl, count, m->qwl, q16(m->qwl), s));
             VRT_TRY(gemm8(kGemmStore, b->Qq_hi, b->Qq_lo, d, m->qwl, b->o, nullptr));
@@ -2459,7 +2577,10 @@ int vrt_tp_unique_id(void* h_out128) {
     return VRT_OK;
 }
 
-int vrt_batch_create(vrt_model* m, uint32_t max_seqs, uint32_t max_positions, int keep_logits, vrt_batch** out) {
+}  // extern "C": reopened after the shared part of batch creation
+
+static int batch_create(vrt_model* m, uint32_t max_seqs, uint32_t max_positions, int keep_logits, bool kv8,
+                        vrt_batch** out) {
     clear_error();
     if (!m || !out) return fail(VRT_E_INVALID, "null argument");
     *out = nullptr;
@@ -2479,11 +2600,22 @@ int vrt_batch_create(vrt_model* m, uint32_t max_seqs, uint32_t max_positions, in
     b->P = max_positions;
     b->out_cap = max_positions;
     b->keep_logits = keep_logits != 0;
+    b->kv8 = kv8;
     const auto& c = m->cfg;
     const uint64_t S = max_seqs, d = c.embedding_length, hd = c.head_dim;
     b->max_splits = std::min<uint32_t>(32u, kAttnWarps * c.head_dim);
     std::vector<uint64_t> sizes;  // bytes, 256-aligned pieces in this order
     for (uint32_t l = 0; l < c.block_count; ++l) {
+        if (kv8) {
+            const uint64_t pages = S * batch_kv8_pages(m, l, max_positions);
+            sizes.push_back(pages * m->KVl * kKv8Page * hd);  // K codes
+            sizes.push_back(pages * m->KVl * kKv8Page * hd);  // V codes
+            sizes.push_back(pages * m->KVl * 4);              // scales
+            sizes.push_back(pages * m->KVl * 4);
+            sizes.push_back(S * m->KVl * kKv8Page * hd * 4);  // tails
+            sizes.push_back(S * m->KVl * kKv8Page * hd * 4);
+            continue;
+        }
         const uint32_t cap = m->layers[l].global ? max_positions : std::min(c.sliding_window, max_positions);
         b->cap.push_back(cap);
         sizes.push_back(S * m->KVl * cap * hd * 4);  // K
@@ -2500,6 +2632,13 @@ int vrt_batch_create(vrt_model* m, uint32_t max_seqs, uint32_t max_positions, in
                               S * xw * 2, S * xw * 2, S * m->ffl * 2, S * m->ffl * 2,
                               Sp * kmax, Sp * kmax, kmax / 32 * Sp * 4, S * m->qwl * 4, S * m->ffl * 4};
     for (auto x : fixed) sizes.push_back(x);
+    const uint64_t pps = (max_positions + kKv8Page - 1) / kKv8Page;
+    if (kv8) {
+        for (uint64_t x : {S * pps * 4, S * pps * 4, S * 4, uint64_t(16), S * m->qwl * 4, S * m->kwl * 4, S * m->kwl * 4,
+                           batch_kv8_workspace(m, max_seqs, max_positions)}) {
+            sizes.push_back(x);
+        }
+    }
     uint64_t total = 0;
     for (auto x : sizes) total += align256(x);
     VRT_CUDA(cudaMalloc(&b->mem, total));
@@ -2512,6 +2651,21 @@ int vrt_batch_create(vrt_model* m, uint32_t max_seqs, uint32_t max_positions, in
         return q;
     };
     for (uint32_t l = 0; l < c.block_count; ++l) {
+        if (kv8) {
+            Kv8View v{};
+            v.kv = m->KVl;
+            v.pages = static_cast<uint32_t>(S * batch_kv8_pages(m, l, max_positions));
+            v.max_seqs = max_seqs;
+            v.pps = static_cast<uint32_t>(pps);
+            v.k = reinterpret_cast<int8_t*>(take());
+            v.v = reinterpret_cast<int8_t*>(take());
+            v.k_scale = reinterpret_cast<float*>(take());
+            v.v_scale = reinterpret_cast<float*>(take());
+            v.k_tail = take();
+            v.v_tail = take();
+            b->kv8_layer.push_back(v);
+            continue;
+        }
         b->kc.push_back(reinterpret_cast<float*>(take()));
         b->vc.push_back(reinterpret_cast<float*>(take()));
     }
@@ -2532,6 +2686,25 @@ int vrt_batch_create(vrt_model* m, uint32_t max_seqs, uint32_t max_positions, in
     b->q_sx = reinterpret_cast<float*>(take());
     b->att32 = reinterpret_cast<float*>(take());
     b->act32 = reinterpret_cast<float*>(take());
+    if (kv8) {
+        int32_t* tables[2];  // sliding, global
+        for (auto& t : tables) t = reinterpret_cast<int32_t*>(take());
+        b->kv8_len = reinterpret_cast<int32_t*>(take());
+        b->kv8_meta = reinterpret_cast<int32_t*>(take());
+        b->kv8_q = reinterpret_cast<float*>(take());
+        b->kv8_k = reinterpret_cast<float*>(take());
+        b->kv8_v = reinterpret_cast<float*>(take());
+        b->kv8_ws = take();
+        std::vector<int32_t> host(S * pps);
+        for (uint32_t l = 0; l < c.block_count; ++l) b->kv8_layer[l].table = tables[m->layers[l].global ? 1 : 0];
+        for (int global = 0; global < 2; ++global) {
+            const uint64_t ring = global ? pps : std::min<uint64_t>(pps, kv8_ring_pages(c.sliding_window));
+            for (uint64_t q = 0; q < S; ++q)
+                for (uint64_t j = 0; j < pps; ++j) host[q * pps + j] = static_cast<int32_t>(q * ring + j % ring);
+            VRT_CUDA(cudaMemcpyAsync(tables[global], host.data(), host.size() * 4, cudaMemcpyHostToDevice, m->ctx->stream));
+            VRT_CUDA(cudaStreamSynchronize(m->ctx->stream));  // `host` is written again
+        }
+    }
     VRT_TRY(make_f16_tmap(&b->xd_hi, b->xh, S, d, 16));
     VRT_TRY(make_f16_tmap(&b->xd_lo, b->xl, S, d, 16));
     VRT_TRY(make_f16_tmap(&b->xq_hi, b->xh, S, m->qwl, 16));
@@ -2560,6 +2733,16 @@ int vrt_batch_create(vrt_model* m, uint32_t max_seqs, uint32_t max_positions, in
     return VRT_OK;
 }
 
+extern "C" {
+
+int vrt_batch_create(vrt_model* m, uint32_t max_seqs, uint32_t max_positions, int keep_logits, vrt_batch** out) {
+    return batch_create(m, max_seqs, max_positions, keep_logits, false, out);
+}
+
+int vrt_batch_create_kv8(vrt_model* m, uint32_t max_seqs, uint32_t max_positions, int keep_logits, vrt_batch** out) {
+    return batch_create(m, max_seqs, max_positions, keep_logits, true, out);
+}
+
 int vrt_batch_destroy(vrt_batch* b) {
     batch_free(b);
     return VRT_OK;
@@ -2583,7 +2766,11 @@ int vrt_batch_prefill(vrt_batch* b, uint32_t seq, const uint32_t* h_prompt, uint
     VRT_CUDA(cudaMemsetAsync(&m->st->status, 0, 4, s));
     SeqTarget t;
     t.prompt = b->prompt;
-    for (uint32_t l = 0; l < c.block_count; ++l) {
+    if (b->kv8) {
+        t.kv8 = b;
+        t.seq = seq;
+    }
+    for (uint32_t l = 0; l < c.block_count && !b->kv8; ++l) {
         const uint64_t off = static_cast<uint64_t>(seq) * m->KVl * b->cap[l] * c.head_dim;
         t.kc.push_back(b->kc[l] + off);
         t.vc.push_back(b->vc[l] + off);

@@ -195,14 +195,16 @@ __global__ void batch_finalize_kernel(unsigned long long* keys, uint32_t* tokens
     pos[s] = first_pos ? first_pos : pos[s] + 1;
 }
 
-// Token m of the chunk (position p0 + m): q heads and k heads -> per-head
-// RMSNorm + RoPE -> q [n][H][hd], k [n][KV][hd]; v copied to v [n][KV][hd].
+// Token m of the chunk (position p0 + m, or pos_of[m] when given, and then
+// len[m] = position + 1): q heads and k heads -> per-head RMSNorm + RoPE ->
+// q [n][H][hd], k [n][KV][hd]; v copied to v [n][KV][hd].
 template <int M>
 __global__ void qk_rope_rows_kernel(const float* qkv, uint32_t H, uint32_t KV, const float* q_norm,
                                     const float* k_norm, const float* rope_cos, const float* rope_sin, uint32_t p0,
-                                    float eps, float* q, float* k, float* v) {
+                                    const uint32_t* pos_of, int32_t* len, float eps, float* q, float* k, float* v) {
     constexpr uint32_t HD = M * 32;
-    const uint32_t m = blockIdx.x, pos = p0 + m;
+    const uint32_t m = blockIdx.x, pos = pos_of ? pos_of[m] : p0 + m;
+    if (len && threadIdx.x == 0) len[m] = static_cast<int32_t>(pos + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
     const float* row = qkv + static_cast<uint64_t>(m) * (H + 2 * KV) * HD;
     const float* cs = rope_cos + static_cast<uint64_t>(pos) * (HD / 2);

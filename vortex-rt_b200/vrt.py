@@ -123,6 +123,7 @@ _SIGS = {
     "vrt_kv8_decode": (_i, [_vp, _vp, _vp, _vp, _u64, _vp, _u32, _u32, _vp, _u64, _vp, _vp, _u64, _vp]),
     "vrt_kv8_prefill": (_i, [_vp, _vp, _vp, _vp, _u64, _vp, _vp, _u32, _u32, _u32, _vp, _u64, _vp, _vp, _u64, _vp]),
     "vrt_batch_create": (_i, [_vp, _u32, _u32, _i, _vp]),
+    "vrt_batch_create_kv8": (_i, [_vp, _u32, _u32, _i, _vp]),
     "vrt_batch_destroy": (_i, [_vp]),
     "vrt_batch_prefill": (_i, [_vp, _u32, _vp, _u32]),
     "vrt_batch_decode_steps": (_i, [_vp, _u32, _u32]),
@@ -351,14 +352,17 @@ class Model:
 
 
 class Batch:
-    """Independent sequences decoded together on one model (vrt_batch_*)."""
+    """Independent sequences decoded together on one model (vrt_batch_*);
+    kv8: with the 8-bit KV cache."""
 
-    def __init__(self, model: "Model", max_seqs: int, max_positions: int, keep_logits: bool = False):
+    def __init__(self, model: "Model", max_seqs: int, max_positions: int, keep_logits: bool = False,
+                 kv8: bool = False):
         self.model = model
         self.h = _vp()
         model.ctx._adopt(self)
         model._batches.add(self)
-        check(lib().vrt_batch_create(model.h, max_seqs, max_positions, int(keep_logits), C.byref(self.h)))
+        create = lib().vrt_batch_create_kv8 if kv8 else lib().vrt_batch_create
+        check(create(model.h, max_seqs, max_positions, int(keep_logits), C.byref(self.h)))
 
     def close(self):
         if self.h and not sys.is_finalizing():  # at interpreter exit the CUDA runtime may already be gone
