@@ -430,7 +430,7 @@ int vrt_kv8_workspace(vrt_ctx* ctx, const vrt_kv8_cache* cache, uint32_t heads, 
     if (!ctx) return fail(VRT_E_INVALID, "kv8: null context");
     const int sms = ctx->prop.multiProcessorCount;
     // of a single row each, either kernel may be meant
-    *bytes = kv8_prefill_workspace(sms, cache->head_dim, cache->kv_heads, heads, count, max_new, max_len);
+    *bytes = kv8_prefill_workspace(sms, cache->head_dim, cache->dtype, cache->kv_heads, heads, count, max_new, max_len);
     if (max_new == 1) {
         *bytes = std::max(*bytes, kv8_decode_workspace(sms, cache->head_dim, cache->kv_heads, heads, count, max_len));
     }

@@ -235,8 +235,10 @@ cudaError_t kv8_append(const Kv8Append& p, uint32_t hd, int dtype, uint32_t coun
 cudaError_t kv8_join(const Kv8Split& p, uint32_t hd, int dtype, cudaStream_t s);
 cudaError_t kv8_decode(const Kv8Attn& p, uint32_t hd, int sms, void* workspace, cudaStream_t s);
 cudaError_t kv8_prefill(const Kv8Attn& p, uint32_t hd, int sms, void* workspace, cudaStream_t s);
-uint64_t kv8_prefill_workspace(int sms, uint32_t hd, uint32_t kv, uint32_t heads, uint32_t count, uint32_t max_new,
-                               uint32_t max_len);
+uint64_t kv8_prefill_workspace(int sms, uint32_t hd, int dtype, uint32_t kv, uint32_t heads, uint32_t count,
+                               uint32_t max_new, uint32_t max_len);
+cudaError_t kv8_prefill_tc(const Kv8Split& p, uint32_t hd, cudaStream_t s);
+uint32_t kv8_prefill_tc_rows(uint32_t hd);  // rows of one of its CTAs
 uint64_t kv8_decode_workspace(int sms, uint32_t hd, uint32_t kv, uint32_t heads, uint32_t count, uint32_t max_len);
 
 }  // namespace vrt

@@ -110,7 +110,8 @@ __global__ void __launch_bounds__(kKpThreads) kv8_prefill_kernel(const Kv8Split 
         for (int d = 0; d < HD / 2; d += 8) {
             float x[8];
             load_row<T, 8>(q + d, x);
-            __half hi[8], lo[8];
+            __align__(16) __half hi[8];
+            __align__(16) __half lo[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) split_f16(live ? x[e] * mul : 0.0f, hi[e], lo[e]);
             *reinterpret_cast<uint4*>(qs + r * Shape::kQ + half + d) = *reinterpret_cast<const uint4*>(hi);
@@ -377,26 +378,37 @@ cudaError_t kv8_join(const Kv8Split& p, uint32_t hd, int dtype, cudaStream_t s) 
 // two CTAs an SM, kKpMinPages pages each at least.
 constexpr uint32_t kKpMinPages = 8;
 
+// Query tokens of a CTA, and whether the tcgen05 form runs: for 16-bit rows,
+// when a sequence may bring more rows than one tile of the warp form has.
+static bool kp_tile(uint32_t hd, int dtype, uint32_t group, uint32_t max_new, uint32_t& tile) {
+    const bool tc = dtype != VRT_F32 && static_cast<uint64_t>(max_new) * group > kKpRows;
+    tile = tc ? kv8_prefill_tc_rows(hd) / 128 * (128 / group) : kKpRows / group;
+    return tc;
+}
+
 static uint64_t kp_cap(int sms, uint32_t tile, uint32_t kv, uint32_t count, uint32_t max_new) {
     const uint64_t ctas = (static_cast<uint64_t>(max_new) + tile - 1) / tile * kv * std::max(1u, count);
     const uint64_t want = std::min<uint64_t>(2ull * sms / std::max<uint64_t>(1, ctas), kKv8MaxSplits);
     return max_new > 65535u ? 1 : std::max<uint64_t>(1, std::min<uint64_t>(want, 65535u / std::max(1u, count)));  // grid limits
 }
 
-static void kp_plan(int sms, const Kv8Attn& a, uint32_t& tile, uint32_t& chunk, uint32_t& splits) {
-    tile = kKpRows / (a.H / a.c.kv);
+static bool kp_plan(int sms, uint32_t hd, const Kv8Attn& a, uint32_t& tile, uint32_t& chunk, uint32_t& splits) {
+    const bool tc = kp_tile(hd, a.dtype, a.H / a.c.kv, a.max_new, tile);
     const uint64_t pages = (static_cast<uint64_t>(a.max_len) + kKv8Page - 1) / kKv8Page;
     const uint64_t cap = kp_cap(sms, tile, a.c.kv, a.count, a.max_new);
     const uint64_t c = std::max<uint64_t>((pages + cap - 1) / cap, kKpMinPages);
     chunk = static_cast<uint32_t>(c);
     splits = static_cast<uint32_t>((pages + c - 1) / c);
+    return tc;
 }
 
 // For any max_len up to this one, as in kv8_decode_workspace.
-uint64_t kv8_prefill_workspace(int sms, uint32_t hd, uint32_t kv, uint32_t heads, uint32_t count, uint32_t max_new,
-                               uint32_t max_len) {
+uint64_t kv8_prefill_workspace(int sms, uint32_t hd, int dtype, uint32_t kv, uint32_t heads, uint32_t count,
+                               uint32_t max_new, uint32_t max_len) {
+    uint32_t tile;
+    kp_tile(hd, dtype, heads / kv, max_new, tile);
     const uint64_t pages = (static_cast<uint64_t>(max_len) + kKv8Page - 1) / kKv8Page;
-    const uint64_t splits = std::min<uint64_t>(kp_cap(sms, kKpRows / (heads / kv), kv, count, max_new),
+    const uint64_t splits = std::min<uint64_t>(kp_cap(sms, tile, kv, count, max_new),
                                                (pages + kKpMinPages - 1) / kKpMinPages);
     return splits > 1 ? static_cast<uint64_t>(count) * max_new * heads * splits * (hd + 2) * 4 : 0;
 }
@@ -427,9 +439,10 @@ static cudaError_t kp_launch(const Kv8Split& p, cudaStream_t s) {
 cudaError_t kv8_prefill(const Kv8Attn& a, uint32_t hd, int sms, void* workspace, cudaStream_t s) {
     Kv8Split p{};
     p.a = a;
-    kp_plan(sms, a, p.tile, p.chunk, p.splits);
+    const bool tc = kp_plan(sms, hd, a, p.tile, p.chunk, p.splits);
     p.part = static_cast<float*>(workspace);
     p.part_ml = p.part + static_cast<uint64_t>(a.count) * a.max_new * a.H * p.splits * hd;
+    if (tc) return kv8_prefill_tc(p, hd, s);
 #define VRT_KP(HD)                                                                \
     if (hd == HD) {                                                               \
         if (a.dtype == VRT_F16) return kp_launch<__half, HD, 1>(p, s);            \

@@ -1827,7 +1827,7 @@ static uint64_t batch_kv8_workspace(const vrt_model* m, uint32_t max_seqs, uint3
     uint64_t most = 16;
     for (uint32_t n = 1; n <= max_seqs; ++n) most = std::max(most, kv8_decode_workspace(sms, hd, m->KVl, m->Hl, n, positions));
     for (uint32_t n = 1; n <= std::min(chunk, positions); ++n)
-        most = std::max(most, kv8_prefill_workspace(sms, hd, m->KVl, m->Hl, 1, n, positions));
+        most = std::max(most, kv8_prefill_workspace(sms, hd, VRT_F32, m->KVl, m->Hl, 1, n, positions));
     return most;
 }
 
