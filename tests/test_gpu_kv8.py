@@ -116,8 +116,8 @@ class Cache:
         magnitudes), scaled, capped (tanh within 4 steps of the cap) and rounded; a weight exp(s) is then off by twice
         the largest score error, and by half an fp16 step where weights are fp16 operands (16-bit types), which are
         kept to 2^-39 of the largest weight, 1 (2^14 times them is held, and fp16 ends at 2^-25), or, where they are
-        multiplied by their page's value scale, to 2^-36 of the largest with the largest scale (held times 2^11 while
-        the largest weight is at most 2^4 above 1); sums over
+        multiplied by their page's value scale, to 2^-28 of the largest with the largest scale (held times 2^3 while
+        the largest weight is at most 2^12 above 1); sums over
         the keys add a step for each; the stored value half a step of its type (below the smallest normal number,
         2^-14 in fp16, a step is finfo.tiny * finfo.eps whatever the value: half of it is added)."""
         k, v = self.values(i)
@@ -147,7 +147,7 @@ class Cache:
         if self.dtype == "f32":
             tol = tol + 2.0 ** -39 * torch.where(torch.isfinite(vz), vz.abs(), 0.0).sum(0)
         elif n:
-            tol = tol + 2.0 ** -36 * n * vv.nan_to_num(0, 0, 0).abs().max()
+            tol = tol + 2.0 ** -28 * n * vv.nan_to_num(0, 0, 0).abs().max()
         return out, lse, tol, ds + (n + 16) * u + lse.abs().nan_to_num(0, 0, 0) * u
 
     def workspace(self, new, most):
