@@ -408,13 +408,31 @@ def test_non_finite_in_sight(ctx, dtype, which):
     out, _ = c.decode(q)
     assert torch.isfinite(out[0, :2]).all() and torch.isnan(out[0, 2:]).all()
     q = c.queries(200, g)
-    for window in (0, 20):
-        out, _ = c.prefill(q, [200], window=window)
+    for window, cap in ((0, 0.0), (20, 0.0), (0, 25.0), (1, 25.0)):
+        out, _ = c.prefill(q, [200], window=window, cap=cap)
         sees = torch.arange(200) >= 96
         if window:
             sees &= torch.arange(200) <= 127 + window - 1
         assert torch.equal(torch.isnan(out).all(2).cpu(), sees[:, None] & torch.tensor([False, False, True, True]))
         assert torch.equal(torch.isnan(out).any(2).cpu(), sees[:, None] & torch.tensor([False, False, True, True]))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+@pytest.mark.parametrize("window", [0, 1, 2])
+def test_nan_query(ctx, dtype, cap, window):
+    """A NaN in a query gives NaN in its own token and head alone, whatever the key that it sees."""
+    c = Cache(ctx, (8, 2, 64), dtype, [130])
+    g = fill(c, [130])
+    q = c.queries(130, g)
+    q[17, 3, 5] = q[38, 0, 63] = q[127, 7, 0] = math.nan
+    bad = torch.zeros((130, 8), dtype=torch.bool, device="cuda")
+    bad[17, 3] = bad[38, 0] = bad[127, 7] = True
+    out, lse = c.prefill(q, [130], window=window, cap=cap)
+    assert torch.equal(torch.isnan(out).all(2), bad) and torch.equal(torch.isnan(out).any(2), bad)
+    assert torch.equal(torch.isnan(lse), bad)
+    out, lse = c.decode(q[127:128], window=window, cap=cap)
+    assert torch.equal(torch.isnan(out).all(2), bad[127:128]) and torch.equal(torch.isnan(out).any(2), bad[127:128])
 
 
 def test_out_of_range(ctx):

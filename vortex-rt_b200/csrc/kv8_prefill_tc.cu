@@ -16,7 +16,7 @@
 //                   (exact) into the 128B-swizzled K-major operand tiles; value
 //                   pages lie [dim][token], which is V^T, the K-major form of
 //                   the second product;
-//   last warpgroup  its first warp issues the MMAs.
+//   last warpgroup  a warp for each row tile issues its MMAs.
 //
 // Scales: a page's key scale and the row's factor are one FMA in front of the
 // exponential.  A page's value scale cannot be taken out of O, which sums over
@@ -33,6 +33,7 @@
 
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 #include "gemm_q8t.cuh"
 #include "kv8.cuh"
@@ -150,6 +151,35 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     return r;
 }
 
+// 2^x of two x <= 100 on the FMA pipe: 2^x = 2^n 2^f with n the nearest whole
+// number (the low bits of x + 1.5 * 2^23) and f in [-1/2, 1/2], 2^f by the
+// polynomial of degree 4 with the smallest relative error there (2^-18.5; a
+// Lawson fit), n added to the exponent field.  From -126 down (-inf too) the
+// result is some 2^-126, and NaN is lost.  For capped scores, which take two
+// special functions (8 cycles a warp each) before their exponential: 4x2048
+// capped 176 -> 98 us.  For plain scores a quarter or half of the exponentials
+// done so changed nothing or cost 5%.
+__device__ __forceinline__ void ex2_fma(float& x, float& y) {
+    const uint64_t v = pair(fmaxf(x, -126.0f), fmaxf(y, -126.0f));
+    const uint64_t r = add2(v, pair(12582912.0f, 12582912.0f));
+    const uint64_t f = fma2(add2(r, pair(-12582912.0f, -12582912.0f)), pair(-1.0f, -1.0f), v);
+    uint64_t q = fma2(f, pair(0.009570101276040077f, 0.009570101276040077f), pair(0.05591785907745361f, 0.05591785907745361f));
+    q = fma2(f, q, pair(0.240247443318367f, 0.240247443318367f));
+    q = fma2(f, q, pair(0.6931217908859253f, 0.6931217908859253f));
+    q = fma2(f, q, pair(0.9999992847442627f, 0.9999992847442627f));
+    float r0, r1, q0, q1;
+    unpair(r, r0, r1);
+    unpair(q, q0, q1);
+    x = __uint_as_float((__float_as_uint(r0) << 23) + __float_as_uint(q0));
+    y = __uint_as_float((__float_as_uint(r1) << 23) + __float_as_uint(q1));
+}
+
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack_rows(float a, float b);
 template <>
@@ -216,10 +246,9 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
     uint64_t* q_full = v_empty + ST;
     uint64_t* s_full = q_full + 1;   // [tile][2] S buffer computed
     uint64_t* p_full = s_full + 4;   // [tile][2] P in its place
-    uint64_t* o_full = p_full + 4;   // [tile] P V added; read at most one phase behind, as a parity tells no more
-    uint64_t* o_last = o_full + 2;   // [tile] the last P V added
-    uint64_t* drained = o_last + 2;  // after a wait gave up: the MMAs in flight are done
-    TcMeta* meta = reinterpret_cast<TcMeta*>(drained + 1);           // [4][PG]
+    uint64_t* o_last = p_full + 4;   // [tile][2] the last P V but one and the last are added
+    uint64_t* drained = o_last + 4;  // [tile] after a wait gave up: the MMAs in flight are done
+    TcMeta* meta = reinterpret_cast<TcMeta*>(drained + 2);           // [4][PG]
     float* reference = reinterpret_cast<float*>(meta + 4 * PG);     // [4 warps], then the value scale that O counts in
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(reference + 5);
     volatile int* missing = reinterpret_cast<volatile int*>(tmem_slot + 1);  // a page was not in the pool
@@ -254,20 +283,17 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
     if (tid == 0) {
         for (int s = 0; s < ST; ++s) {
             mbar_init(k_full + s, 4);
-            mbar_init(k_empty + s, 1);
+            mbar_init(k_empty + s, MT);
             mbar_init(v_full + s, 4);
-            mbar_init(v_empty + s, 1);
+            mbar_init(v_empty + s, MT);
         }
         mbar_init(q_full, 4 * MT);
-        mbar_init(drained, 1);
         for (int b = 0; b < 4; ++b) {
             mbar_init(s_full + b, 1);
             mbar_init(p_full + b, 4);
+            mbar_init(o_last + b, 1);
         }
-        for (int t = 0; t < 2; ++t) {
-            mbar_init(o_full + t, 1);
-            mbar_init(o_last + t, 1);
-        }
+        for (int t = 0; t < 2; ++t) mbar_init(drained + t, 1);
         *missing = 0;
         fence_mbar_init();
     }
@@ -293,14 +319,17 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
         {
             const T* q = static_cast<const T*>(p.a.q) + at * p.a.q_stride + static_cast<uint64_t>(live ? h : g * R) * HD;
             float m = 0.0f;
+            bool finite = true;
 #pragma unroll 2
             for (int d = 0; d < HD; d += 8) {
                 float x[8];
                 load_row<T, 8>(q + d, x);
                 m = fmaxf(m, max_abs(x));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) finite = finite && fabsf(x[e]) < INFINITY;
             }
             const float mul = kv8_row_unit(m);
-            unit = 1.0f / mul * fabsf(p.a.scale);
+            unit = finite ? 1.0f / mul * fabsf(p.a.scale) : NAN;
             const float sign = live ? (p.a.scale < 0.0f ? -mul : mul) : 0.0f;
 #pragma unroll 2
             for (int d = 0; d < HD; d += 8) {
@@ -340,27 +369,31 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
             tmem_fetch32(s_col + 32, vb);
             const TcMeta* mt = meta + (j / SUB & 3) * PG + j % SUB * 2;
             float a0 = mt[0].k_scale * factor, a1 = mt[1].k_scale * factor, b0 = mt[0].v_log, b1 = mt[1].v_log;
+            // a score times a plus b is the exponent of its weight times the value scale, inv takes that back for the
+            // sum; a NaN (of a page's scales, or of the query in `factor`) reaches the sum, and so the row, through inv
+            float i0v = mt[0].v_inv, i1v = mt[1].v_inv;
             const int i0p = static_cast<int>(j0) + 2 * j;
             const bool whole = (i0p + 1 < whole_a || (i0p >= whole_b && i0p + 1 < whole_c)) && !*missing;
             tmem_arrived(va, vb);
             if (!whole) {
-                // Takes a page's scores to what the row sees; a score times a plus b is its weight's exponent.  What
-                // the row does not see is -inf, so the factor is kept above 0 and a NaN scale goes into the scores.
-                auto mask = [&](int c, uint32_t(&v)[32], float& a, float& b) {
+                // Takes a page's scores to what the row sees: the rest is -inf, so the factor is kept above 0, and a NaN
+                // scale of a page that the row does not see is left out.
+                auto mask = [&](int c, uint32_t(&v)[32], float& a, float& b, float& inv) {
                     const int t0 = static_cast<int>(span.page(j0 + 2 * j + c) * kKv8Page);
                     auto below = [](int x) { return x >= 32 ? 0xffffffffu : x <= 0 ? 0u : (1u << x) - 1u; };
                     const uint32_t see = mt[c].there ? ((below(end - t0) & ~below(lo - t0)) | below(prefix - t0)) : 0u;
                     const bool bad = !(a < INFINITY) || !(b <= 0.0f);
                     a = bad ? 1.0f : fmaxf(a, 1e-37f);
                     b = bad ? 0.0f : b;
+                    inv = bad ? (see ? NAN : 1.0f) : inv;
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const uint32_t x = bad ? 0x7fffffffu : v[i];
-                        v[i] = see >> i & 1 ? x : 0xff800000u;
-                    }
+                    for (int i = 0; i < 32; ++i) v[i] = see >> i & 1 ? v[i] : 0xff800000u;
                 };
-                mask(0, va, a0, b0);
-                mask(1, vb, a1, b1);
+                mask(0, va, a0, b0, i0v);
+                mask(1, vb, a1, b1, i1v);
+            } else {
+                i0v = a0 < INFINITY ? i0v : NAN;
+                i1v = a1 < INFINITY ? i1v : NAN;
             }
             auto highest = [&](const uint32_t(&v)[32], float a) {
                 float m4[4];
@@ -381,7 +414,9 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
                 if (grown) mx = top;
                 sum *= f;
                 if (j > 0) {
-                    ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded(o_full + t, (j - 1) & 1));
+                    // P V of key tile j - 1 is done when S of j + 1, issued behind it, is
+                    uint64_t* added = j + 1 < mine ? s_full + 2 * t + ((j + 1) & 1) : o_last + 2 * t;
+                    ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded(added, j + 1 < mine ? ((j + 1) >> 1) & 1 : 0));
                     if (!ok) break;
                     tc_fence_after();
 #pragma unroll 1
@@ -400,34 +435,50 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
                 }
             }
             const float base = kTcLift - (mx == -INFINITY ? 0.0f : mx);
-            auto weigh = [&](int c, const uint32_t(&v)[32], float a, float b) {
+            // kHidden: scores of -inf among them, which a tanh would make finite
+            auto weigh = [&](int c, const uint32_t(&v)[32], float a, float b, float inv, auto kHidden) {
                 uint32_t w[16];
                 b += base;
+                // CAP: cap * tanh(y) = cap - 2 cap / (e^2y + 1)
+                const float ca = a * (inv_cap * 2.0f * kLog2e), c1 = p.a.softcap * kLog2e + b, c2 = -2.0f * kLog2e * p.a.softcap;
                 const uint64_t a2 = pair(a, a), b2 = pair(b, b);
                 uint64_t part[2] = {0, 0};
 #pragma unroll
                 for (int e = 0; e < 32; e += 2) {
                     float x = __uint_as_float(v[e]), y = __uint_as_float(v[e + 1]);
-                    if (CAP) {  // tanh(-inf) is -1
-                        x = x == -INFINITY ? x : capped<false>(x * a, p.a.softcap, inv_cap) + b;
-                        y = y == -INFINITY ? y : capped<false>(y * a, p.a.softcap, inv_cap) + b;
+                    if (CAP) {
+                        const float s0 = x, s1 = y;
+                        x = fmaf(rcp_approx(ex2(x * ca) + 1.0f), c2, c1);
+                        y = fmaf(rcp_approx(ex2(y * ca) + 1.0f), c2, c1);
+                        if (decltype(kHidden)::value) {
+                            x = s0 == -INFINITY ? s0 : x;
+                            y = s1 == -INFINITY ? s1 : y;
+                        }
                     } else {
                         unpair(fma2(pair(x, y), a2, b2), x, y);
                     }
-                    x = ex2(x);
-                    y = ex2(y);
+                    if (CAP) {  // two special functions are spent on the tanh already
+                        ex2_fma(x, y);
+                    } else {
+                        x = ex2(x);
+                        y = ex2(y);
+                    }
                     part[e >> 1 & 1] = add2(part[e >> 1 & 1], pair(x, y));
                     const __half2 hh = __floats2half2_rn(x, y);
                     w[e / 2] = *reinterpret_cast<const uint32_t*>(&hh);
                 }
                 float x, y;
                 unpair(add2(part[0], part[1]), x, y);
-                x += y;
-                if (x != 0.0f) sum = fmaf(x, mt[c].v_inv, sum);  // a page that the row does not see may have any scale
+                sum = fmaf(x + y, inv, sum);
                 tmem_st16(s_col + 16 * c, w);
             };
-            weigh(0, va, a0, b0);
-            weigh(1, vb, a1, b1);
+            if (CAP && !whole) {
+                weigh(0, va, a0, b0, i0v, std::true_type{});
+                weigh(1, vb, a1, b1, i1v, std::true_type{});
+            } else {
+                weigh(0, va, a0, b0, i0v, std::false_type{});
+                weigh(1, vb, a1, b1, i1v, std::false_type{});
+            }
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
@@ -435,9 +486,10 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
         }
         // ---- output
         if (mine > 0) {
-            ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded(o_last + t, 0));
+            ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded(o_last + 2 * t + 1, 0));
             tc_fence_after();
         }
+        if (mx == -INFINITY && sum < INFINITY) sum = 0.0f;  // nothing seen: what ex2_fma makes of -inf
         const float ref = mine > 0 ? reference[4] : 0.0f;
         const float mul = used == 1 ? (sum == 0.0f ? 0.0f : ref / sum) : ref;
         T* out = static_cast<T*>(p.a.out) + at * p.a.out_stride + static_cast<uint64_t>(h) * HD;
@@ -582,67 +634,62 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
     } else {
         // -------------------------------------------- MMA, as a whole warp: see warp_mma_ss
         fewer_registers<Shape::kRegsMma>();
-        if (warp == 4 * MT + 8) {
+        const int t = warp - (4 * MT + 8);
+        if (t < MT) {
             auto wait = [&](uint64_t* bar, int phase) { ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded(bar, phase & 1)); };
+            const int mine = t ? need[1] : need[0];
             int k_seen = -1, v_seen = -1;  // blocks waited for
-            const int need0 = need[0], need1 = need[1];
-            // whether no MMA of the same kind that comes after row tile t's key tile j reads its block: they come by key
-            // tile, then by row tile
-            auto last_use = [&](int t, int j) {
-                const int stop = (j / SUB + 1) * SUB, own = min(t ? need1 : need0, stop) - 1;
-                const int other = MT == 2 ? min(t ? need0 : need1, stop) - 1 : -1;
-                return j == own && (other < j || (other == j && t == 1));
-            };
-            if (J > 0) wait(q_full, 0);
+            const uint64_t qa = sw128_desc(smem_addr(sq + t * Shape::kQTile));
+            if (mine > 0) wait(q_full, 0);
             // j < 0: only S of the first key tiles
 #pragma unroll 1
-            for (int j = -kLook; j < J && ok; ++j) {
-#pragma unroll
-                for (int t = 0; t < MT; ++t) {
-                    const int mine = t ? need1 : need0;
-                    if (j >= 0 && j < mine && ok) {
-                        const int buf = 2 * t + (j & 1), blk = j / SUB;
-                        wait(p_full + buf, j >> 1);
-                        if (blk > v_seen) {
-                            wait(v_full + blk % ST, blk / ST);
-                            v_seen = blk;
-                        }
-                        if (ok) {
-                            tc_fence_after();
-                            const uint64_t va = sw128_desc(smem_addr(sv + blk % ST * Shape::kKTile) + j % SUB * (HD * 128));
-#pragma unroll
-                            for (int k = 0; k < KT / 16; ++k) {
-                                warp_mma_ts(tmem + Shape::kOCol + t * HD, tmem + buf * KT + k * 8, va + k * 2, kIdescO, j > 0 || k > 0);
-                            }
-                            warp_commit((j + 1 < mine ? o_full : o_last) + t);
-                            if (last_use(t, j)) warp_commit(v_empty + blk % ST);
-                        }
+            for (int j = -kLook; j < mine && ok; ++j) {
+                if (j >= 0) {
+                    const int buf = 2 * t + (j & 1), blk = j / SUB;
+                    wait(p_full + buf, j >> 1);
+                    if (blk > v_seen) {
+                        wait(v_full + blk % ST, blk / ST);
+                        v_seen = blk;
                     }
-                    const int next = j + kLook;
-                    if (next < mine && ok) {
-                        const int buf = 2 * t + (next & 1), blk = next / SUB;
-                        if (blk > k_seen) {
-                            wait(k_full + blk % ST, blk / ST);
-                            k_seen = blk;
-                        }
-                        if (ok) {
-                            tc_fence_after();
-                            const uint64_t qa = sw128_desc(smem_addr(sq + t * Shape::kQTile));
-                            const uint64_t ka = sw128_desc(smem_addr(sk + blk % ST * Shape::kKTile) + next % SUB * (KT * 128));
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t va = sw128_desc(smem_addr(sv + blk % ST * Shape::kKTile) + j % SUB * (HD * 128));
 #pragma unroll
-                            for (int k = 0; k < HD / 16; ++k) {  // descriptors count in 16 bytes
-                                warp_mma_ss(tmem + buf * KT, qa + (k / 4 * (128 * 128) + k % 4 * 32) / 16,
-                                            ka + (k / 4 * (KB * 128) + k % 4 * 32) / 16, kIdescS, k > 0);
-                            }
-                            warp_commit(s_full + buf);
-                            if (last_use(t, next)) warp_commit(k_empty + blk % ST);
-                        }
+                    for (int k = 0; k < KT / 16; ++k) {
+                        warp_mma_ts(tmem + Shape::kOCol + t * HD, tmem + buf * KT + k * 8, va + k * 2, kIdescO, j > 0 || k > 0);
                     }
+                    if (j + 2 >= mine) warp_commit(o_last + 2 * t + (j + 1 == mine));
+                    if (j + 1 == mine || j % SUB == SUB - 1) warp_commit(v_empty + blk % ST);
+                }
+                const int next = j + kLook;
+                if (next < mine) {
+                    const int buf = 2 * t + (next & 1), blk = next / SUB;
+                    if (blk > k_seen) {
+                        wait(k_full + blk % ST, blk / ST);
+                        k_seen = blk;
+                    }
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t ka = sw128_desc(smem_addr(sk + blk % ST * Shape::kKTile) + next % SUB * (KT * 128));
+#pragma unroll
+                    for (int k = 0; k < HD / 16; ++k) {  // descriptors count in 16 bytes
+                        warp_mma_ss(tmem + buf * KT, qa + (k / 4 * (128 * 128) + k % 4 * 32) / 16,
+                                    ka + (k / 4 * (KB * 128) + k % 4 * 32) / 16, kIdescS, k > 0);
+                    }
+                    warp_commit(s_full + buf);
+                    if (next + 1 == mine || next % SUB == SUB - 1) warp_commit(k_empty + blk % ST);
                 }
             }
+            // blocks that only the other row tile reads: given back as they come, so that each counts in its own phase
+            for (int blk = (mine + SUB - 1) / SUB; blk < blocks_k && ok; ++blk) {
+                wait(k_full + blk % ST, blk / ST);
+                if (lane == 0) mbar_arrive(k_empty + blk % ST);
+                wait(v_full + blk % ST, blk / ST);
+                if (lane == 0) mbar_arrive(v_empty + blk % ST);
+            }
             if (!ok) {
-                warp_commit(drained);
-                mbar_wait_bounded(drained, 0);
+                warp_commit(drained + t);
+                mbar_wait_bounded(drained + t, 0);
             }
         }
     }
