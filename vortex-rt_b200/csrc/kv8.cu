@@ -10,23 +10,52 @@
 
 namespace vrt {
 
-constexpr int kKv8Threads = 256;
 
-// x / s rounded half to even.  x * inv is within 127 * 2^-23 of x / s, so its
-// rounding is right unless it falls next to a half; there, and for a scale so
-// small that 1 / s is not finite, a division in 64 bits decides (two 24-bit
-// numbers' quotient is no nearer to a half than 2^-33 unless it is one).
-__device__ __forceinline__ int kv8_code(float x, float s, float inv) {
-    const float t = x * inv;
-    float r = rintf(t);
-    if (!(fabsf(t - r) < 0.4999f)) {
-        r = s > 0.0f ? static_cast<float>(rint(static_cast<double>(x) / static_cast<double>(s))) : 0.0f;
-    }
-    return static_cast<int>(fminf(fmaxf(r, -127.0f), 127.0f));
+// x / s rounded half to even, to a code.  The exact form: two 24-bit numbers'
+// quotient is no nearer to a half than 2^-33 unless it is one, which a
+// division in 64 bits tells apart.
+__device__ __noinline__ int kv8_code_exact(float x, float s) {
+    if (!(s > 0.0f)) return 0;  // a page of zeros, or with a NaN
+    return static_cast<int>(fmin(fmax(rint(static_cast<double>(x) / static_cast<double>(s)), -127.0), 127.0));
 }
 
-__device__ __forceinline__ uint32_t pack4(const int (&q)[4]) {
-    return (q[0] & 0xff) | (q[1] & 0xff) << 8 | (q[2] & 0xff) << 16 | static_cast<uint32_t>(q[3]) << 24;
+__device__ __forceinline__ uint32_t pack_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __byte_perm(__byte_perm(a, b, 0x0040u), __byte_perm(c, d, 0x0040u), 0x5410u);
+}
+
+// Codes of N values, four to a word.  x * inv is within 127 * 2^-24 = 7.6e-6
+// of x / s, so its nearest whole number, the low byte of x * inv + 1.5 * 2^23,
+// is right unless it falls next to a half (then the exact form decides, as it
+// does for a scale so small that 1 / s is not finite).
+template <int N>
+__device__ __forceinline__ void kv8_codes(const float (&x)[N], float s, float inv, uint32_t (&w)[N / 4]) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+        float far = 0.0f, sum = 0.0f;  // the largest distance from the whole number; NaN, if one is
+        uint32_t b[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float m = fmaf(x[i + j], inv, 12582912.0f), d = fmaf(x[i + j], inv, 12582912.0f - m);
+            far = fmaxf(far, fabsf(d));
+            sum += d;
+            b[j] = __float_as_uint(m);
+        }
+        w[i / 4] = pack_bytes(b[0], b[1], b[2], b[3]);
+        if (!(far < 0.49999f && sum == sum)) {
+            w[i / 4] = pack_bytes(kv8_code_exact(x[i], s), kv8_code_exact(x[i + 1], s), kv8_code_exact(x[i + 2], s),
+                                  kv8_code_exact(x[i + 3], s));
+        }
+    }
+}
+
+// Four rows of four bytes -> four columns.
+__device__ __forceinline__ void transpose4(uint32_t (&a)[4]) {
+    const uint32_t lo0 = __byte_perm(a[0], a[1], 0x5140u), lo1 = __byte_perm(a[2], a[3], 0x5140u);
+    const uint32_t hi0 = __byte_perm(a[0], a[1], 0x7362u), hi1 = __byte_perm(a[2], a[3], 0x7362u);
+    a[0] = __byte_perm(lo0, lo1, 0x5410u);
+    a[1] = __byte_perm(lo0, lo1, 0x7632u);
+    a[2] = __byte_perm(hi0, hi1, 0x5410u);
+    a[3] = __byte_perm(hi0, hi1, 0x7632u);
 }
 
 // Pages that n rows touch at most, wherever they start.
@@ -34,15 +63,19 @@ static uint32_t kv8_touched(uint32_t n) { return (n + kKv8Page - 2) / kKv8Page +
 
 // CTA (b, g + kv * {K, V}, i): the b-th page of sequence i that the new rows
 // touch, KV head g.  The page's rows (from the tail below `start`, else from
-// the call) are held in registers, 8 threads a row: maximum, scale, codes.
-// The CTA of a sequence's first page also brings the tail up to date, after
-// it has read it: no other CTA touches that tail.  A page whose scale did not
-// change keeps its old codes, so that a step of one token writes one row.
-// Bound by HBM for prompts, by one round of dependent loads for single rows.
+// the call) are held in registers, 4 threads a row with every fourth 16-byte
+// piece each: maximum, scale, codes.  The CTA of a sequence's first page also
+// brings the tail up to date, after it has read it: no other CTA touches that
+// tail.  A page whose scale did not change keeps its old codes, so that a step
+// of one token writes one row.  Prompts are bound by instructions next to HBM
+// (conversions, maximum and rounding are some 8 a value), single rows by a
+// round of dependent loads.
+constexpr int kKaThreads = 128;
+
 template <typename T, int HD>
-__global__ void __launch_bounds__(kKv8Threads) kv8_append_kernel(const Kv8Append p) {
-    constexpr int N = HD / 8;  // elements of a thread
-    __shared__ uint32_t top[kKv8Threads / 32];
+__global__ void __launch_bounds__(kKaThreads) kv8_append_kernel(const Kv8Append p) {
+    constexpr int P = 16 / sizeof(T), N = HD / 4, C = N / P;  // values of a piece, of a thread; its pieces
+    __shared__ uint32_t top[kKaThreads / 32];
     __shared__ uint32_t tile[kKv8Page * (HD / 4 + 1)];
     const uint32_t g = blockIdx.y % p.c.kv, seq = blockIdx.z;
     const bool is_v = blockIdx.y >= p.c.kv;
@@ -54,20 +87,29 @@ __global__ void __launch_bounds__(kKv8Threads) kv8_append_kernel(const Kv8Append
         if (threadIdx.x == 0) atomicOr(p.status, kStatusKv8Range);
         if (start < 0 || start >= limit) return;
     }
-    const int64_t end = min(start + n, limit);
-    const int64_t first = start / kKv8Page, page = first + blockIdx.x;
-    if (page * kKv8Page >= end) return;
+    // positions are below 2^31 from here on, and row 0 of the page is at `at`
+    const int from = static_cast<int>(start), end = static_cast<int>(min(start + n, limit));
+    const int page = from / static_cast<int>(kKv8Page) + static_cast<int>(blockIdx.x);
+    if (page > (end - 1) / static_cast<int>(kKv8Page)) return;
+    const int id = kv8_page(p.c, seq, static_cast<uint32_t>(page), p.status);
 
     const T* rows = static_cast<const T*>(is_v ? p.v : p.k) + static_cast<uint64_t>(g) * HD;
     T* tail = static_cast<T*>(is_v ? p.c.v_tail : p.c.k_tail) + (static_cast<uint64_t>(seq) * p.c.kv + g) * kKv8Page * HD;
-    const int row = threadIdx.x / 8, col = threadIdx.x % 8 * N;
-    const int64_t pos = page * kKv8Page + row;
+    const int row = threadIdx.x / 4, first = threadIdx.x % 4 * P;
+    const int pos = page * static_cast<int>(kKv8Page) + row;
     float x[N];
     if (pos >= end) {
 #pragma unroll
         for (int i = 0; i < N; ++i) x[i] = 0.0f;
     } else {
-        load_row<T, N>((pos < start ? tail + row * HD : rows + static_cast<uint64_t>(r0 + (pos - start)) * p.stride) + col, x);
+        const T* src = (pos < from ? tail + row * HD : rows + static_cast<uint64_t>(r0 + (pos - from)) * p.stride) + first;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            float y[P];
+            load_row<T, P>(src + c * 4 * P, y);
+#pragma unroll
+            for (int j = 0; j < P; ++j) x[c * P + j] = y[j];
+        }
     }
     // |x| as bits: ordered like the values, infinities and NaN on top
     uint32_t m = 0;
@@ -77,74 +119,72 @@ __global__ void __launch_bounds__(kKv8Threads) kv8_append_kernel(const Kv8Append
     if (threadIdx.x % 32 == 0) top[threadIdx.x / 32] = m;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kKv8Threads / 32; ++w) m = max(m, top[w]);
+    for (int w = 0; w < kKaThreads / 32; ++w) m = max(m, top[w]);
     const float s = m < 0x7f800000u ? __uint_as_float(m) / 127.0f : NAN;
     const float inv = s > 0.0f ? 1.0f / s : 0.0f;
 
     // the tail: new rows of the last page, when that is not full
-    if (blockIdx.x == 0 && end % kKv8Page) {
-        const int64_t lp = end / kKv8Page, at = lp * kKv8Page + row;
-        if (at >= start && at < end) {
-            const uint4* src = reinterpret_cast<const uint4*>(rows + static_cast<uint64_t>(r0 + (at - start)) * p.stride + col);
-            uint4* dst = reinterpret_cast<uint4*>(tail + row * HD + col);
+    if (blockIdx.x == 0 && end % static_cast<int>(kKv8Page)) {
+        const int at = end / static_cast<int>(kKv8Page) * static_cast<int>(kKv8Page) + row;
+        if (at >= from && at < end) {
+            const T* src = rows + static_cast<uint64_t>(r0 + (at - from)) * p.stride + first;
+            T* dst = tail + row * HD + first;
 #pragma unroll
-            for (int i = 0; i < static_cast<int>(N * sizeof(T) / 16); ++i) dst[i] = src[i];
+            for (int c = 0; c < C; ++c) *reinterpret_cast<uint4*>(dst + c * 4 * P) = *reinterpret_cast<const uint4*>(src + c * 4 * P);
         }
     }
 
-    const int id = kv8_page(p.c, seq, static_cast<uint32_t>(page), p.status);
     if (id < 0) return;
     const uint64_t head = static_cast<uint64_t>(id) * p.c.kv + g;
     float* scale = (is_v ? p.c.v_scale : p.c.k_scale) + head;
-    const int64_t kept = page * kKv8Page < start ? start - page * kKv8Page : 0;  // rows that the page already held
-    const bool same = kept > 0 && *scale == s;
-    __syncthreads();  // every thread has read the old scale
+    const int kept = max(0, from - page * static_cast<int>(kKv8Page));  // rows that the page already held
+    bool same = false;
+    if (kept > 0) {
+        same = *scale == s;
+        __syncthreads();  // every thread has read the old scale
+    }
     if (threadIdx.x == 0) *scale = s;
     uint32_t w[N / 4];
-#pragma unroll
-    for (int i = 0; i < N / 4; ++i) {
-        int q[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) q[j] = s >= 0.0f ? kv8_code(x[4 * i + j], s, inv) : 0;
-        w[i] = pack4(q);
-    }
+    kv8_codes<N>(x, s, inv, w);
+    const bool fresh = !same || (row >= kept && pos < end);  // codes of this row are to be written
     if (!is_v) {
-        if (same && (row < kept || pos >= end)) return;
-        uint32_t* dst = reinterpret_cast<uint32_t*>(p.c.k + (head * kKv8Page + row) * HD + col);
-        if constexpr (N == 8) {
-            *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
-        } else {
+        if (!fresh) return;
+        int8_t* dst = p.c.k + (head * kKv8Page + row) * HD + first;
 #pragma unroll
-            for (int i = 0; i < N / 16; ++i)
-                reinterpret_cast<uint4*>(dst)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        for (int c = 0; c < C; ++c) {
+            if constexpr (P == 8) {
+                *reinterpret_cast<uint2*>(dst + c * 4 * P) = make_uint2(w[2 * c], w[2 * c + 1]);
+            } else {
+                *reinterpret_cast<uint32_t*>(dst + c * 4 * P) = w[c];
+            }
         }
         return;
     }
     int8_t* vp = p.c.v + head * HD * kKv8Page;
     if (same) {
-        if (row >= kept && pos < end) {
+        if (!fresh) return;
 #pragma unroll
-            for (int i = 0; i < N; ++i) vp[(col + i) * kKv8Page + row] = static_cast<int8_t>(w[i / 4] >> 8 * (i % 4));
-        }
+        for (int i = 0; i < N; ++i) vp[(i / P * 4 * P + first + i % P) * kKv8Page + row] = static_cast<int8_t>(w[i / 4] >> 8 * (i % 4));
         return;
     }
     // values lie [dim][token]: transposed through shared memory
 #pragma unroll
-    for (int i = 0; i < N / 4; ++i) tile[row * (HD / 4 + 1) + col / 4 + i] = w[i];
+    for (int i = 0; i < N / 4; ++i) tile[row * (HD / 4 + 1) + (i * 4 / P * 4 * P + first + i * 4 % P) / 4] = w[i];
     __syncthreads();
-    const uint8_t* t8 = reinterpret_cast<const uint8_t*>(tile);
-    for (int c = threadIdx.x; c < HD * 2; c += kKv8Threads) {
-        const int d = c % HD, r = c / HD * 16;
-        uint32_t o[4];
+    // four tokens by four dims a thread; the eight lanes of a token group write whole 32-byte sectors
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            o[e] = 0;
+    for (int c = threadIdx.x; c < HD * 2; c += kKaThreads) {
+        const int r = c % 8 * 4, d = c / 8;  // dims 4 d .. 4 d + 3
+        uint32_t a[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) o[e] |= static_cast<uint32_t>(t8[(r + 4 * e + j) * (HD + 4) + d]) << 8 * j;
-        }
-        *reinterpret_cast<uint4*>(vp + d * kKv8Page + r) = make_uint4(o[0], o[1], o[2], o[3]);
+        for (int j = 0; j < 4; ++j) a[j] = tile[(r + j) * (HD / 4 + 1) + d];
+        transpose4(a);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *reinterpret_cast<uint32_t*>(vp + (4 * d + j) * kKv8Page + r) = a[j];
     }
 }
+
+constexpr int kKv8Threads = 256;
 
 // CTA (b, g + kv * {K, V}, i): code * scale of the b-th page that the rows of
 // sequence i touch -> fp32 rows.  Values are transposed in shared memory.
@@ -169,19 +209,24 @@ __global__ void __launch_bounds__(kKv8Threads) kv8_read_kernel(const Kv8Read p) 
     if (id < 0) return;
     const uint64_t head = static_cast<uint64_t>(id) * p.c.kv + g;
     const float s = (is_v ? p.c.v_scale : p.c.k_scale)[head];
-    const uint4* src = reinterpret_cast<const uint4*>((is_v ? p.c.v : p.c.k) + head * kKv8Page * HD);
+    const int8_t* src = (is_v ? p.c.v : p.c.k) + head * kKv8Page * HD;
     for (int c = threadIdx.x; c < HD * 2; c += kKv8Threads) {
-        const uint4 u = src[c];
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        uint32_t w[4];
         if (!is_v) {
-            const int r = c / (HD / 16), d = c % (HD / 16) * 4;
+            const uint4 u = reinterpret_cast<const uint4*>(src)[c];
+            w[0] = u.x;
+            w[1] = u.y;
+            w[2] = u.z;
+            w[3] = u.w;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) tile[r * W + d + e] = w[e];
+            for (int j = 0; j < 4; ++j) tile[c / (HD / 16) * W + c % (HD / 16) * 4 + j] = w[j];
         } else {
-            const int d = c / 2, r = c % 2 * 16;
-            uint8_t* t8 = reinterpret_cast<uint8_t*>(tile);
+            const int r = c % 8 * 4, d = c / 8;  // four tokens by four dims
 #pragma unroll
-            for (int e = 0; e < 16; ++e) t8[(r + e) * (W * 4) + d] = static_cast<uint8_t>(w[e / 4] >> 8 * (e % 4));
+            for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const uint32_t*>(src + (4 * d + j) * kKv8Page + r);
+            transpose4(w);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) tile[(r + j) * W + d] = w[j];
         }
     }
     __syncthreads();
@@ -191,12 +236,13 @@ __global__ void __launch_bounds__(kKv8Threads) kv8_read_kernel(const Kv8Read p) 
         const int r = c / (HD / 4), d = c % (HD / 4);
         const int64_t pos = page * kKv8Page + r;
         if (pos < start || pos >= end) continue;
-        const uint32_t w = tile[r * W + d];
+        // a byte offset by 128 under the exponent of 2^23, less 2^23 + 128: the code, without a conversion
+        const uint32_t w = tile[r * W + d] ^ 0x80808080u;
         float4 f;
-        f.x = static_cast<float>(static_cast<int8_t>(w)) * s;
-        f.y = static_cast<float>(static_cast<int8_t>(w >> 8)) * s;
-        f.z = static_cast<float>(static_cast<int8_t>(w >> 16)) * s;
-        f.w = static_cast<float>(static_cast<int8_t>(w >> 24)) * s;
+        f.x = (__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7550u)) - 8388736.0f) * s;
+        f.y = (__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7551u)) - 8388736.0f) * s;
+        f.z = (__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7552u)) - 8388736.0f) * s;
+        f.w = (__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7553u)) - 8388736.0f) * s;
         reinterpret_cast<float4*>(out + static_cast<uint64_t>(r0 + (pos - start)) * stride)[d] = f;
     }
 }
@@ -204,7 +250,7 @@ __global__ void __launch_bounds__(kKv8Threads) kv8_read_kernel(const Kv8Read p) 
 cudaError_t kv8_append(const Kv8Append& p, uint32_t hd, int dtype, uint32_t count, cudaStream_t s) {
     const dim3 grid(kv8_touched(p.max_new), 2 * p.c.kv, count);
 #define VRT_KA(TY, T, HD) \
-    if (dtype == TY && hd == HD) return launch(kv8_append_kernel<T, HD>, grid, dim3(kKv8Threads), 0, s, false, p);
+    if (dtype == TY && hd == HD) return launch(kv8_append_kernel<T, HD>, grid, dim3(kKaThreads), 0, s, false, p);
 #define VRT_KA3(HD) VRT_KA(VRT_F32, float, HD) VRT_KA(VRT_F16, __half, HD) VRT_KA(VRT_BF16, __nv_bfloat16, HD)
     VRT_KA3(64) VRT_KA3(128) VRT_KA3(256)
 #undef VRT_KA3
