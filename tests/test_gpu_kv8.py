@@ -166,7 +166,7 @@ class Cache:
         torch.cuda.synchronize()
         return out, lse
 
-    def prefill(self, q, new, window=0, prefix=None, cap=0.0, max_len=None, max_new=None):
+    def prefill(self, q, new, window=0, prefix=None, cap=0.0, max_len=None, max_new=None, scale=None):
         cu = torch.tensor(np.cumsum([0] + list(new)), **I32)
         most, mn = max_len or self.pps * PAGE, max_new or max(1, max(new))
         ws, nb = self.workspace(mn, most)
@@ -174,7 +174,7 @@ class Cache:
         ln = torch.tensor(self.lens(), **I32)
         pre = torch.tensor(prefix, **I32) if prefix else None
         self.c.prefill(q.data_ptr(), ln.data_ptr(), cu.data_ptr(), self.n, self.h, out.data_ptr(), max_new=mn,
-                       max_len=most, window=window, softcap=cap, prefix=pre.data_ptr() if prefix else None,
+                       max_len=most, window=window, softcap=cap, scale=scale, prefix=pre.data_ptr() if prefix else None,
                        lse=lse.data_ptr(), workspace=ws.data_ptr(), workspace_bytes=nb, stream=stream())
         torch.cuda.synchronize()
         return out, lse
@@ -371,6 +371,40 @@ def test_decode_extreme_scores(ctx, dtype):
         ro, rl, to, tl = c.expect(0, q, [699])
         near(out, ro, to, f"out at {size}")
         near(lse, rl, tl, f"lse at {size}")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scale,qs,ks", [(-0.2, 1.0, 1.0), (0.0, 1.0, 1.0), (0.1, 1e-3, 1e3), (0.1, 1e4, 1e-4), (1e3, 1e-2, 1e-2)])
+def test_scales(ctx, dtype, scale, qs, ks):
+    """Negative and zero score scales; small queries on large keys and the other way round."""
+    c = Cache(ctx, (8, 2, 64), dtype, [300])
+    g = torch.Generator("cuda").manual_seed(12)
+    c.append([((c.random(300, g).float() * ks).to(TYPES[dtype]), c.random(300, g))])
+    q = (c.queries(150, g).float() * qs).to(TYPES[dtype])
+    for cap in (0.0, 5.0):
+        out, lse = c.prefill(q, [150], cap=cap, scale=scale)
+        ro, rl, to, tl = c.expect(0, q, range(150, 300), cap=cap, scale=scale)
+        near(out, ro, to, "prompt")
+        near(lse, rl, tl, "lse of the prompt")
+        out, lse = c.decode(q[149:], cap=cap, scale=scale)
+        near(out, ro[149:], to[149:], "token")
+        near(lse, rl[149:], tl[149:], "lse of the token")
+
+
+def test_far_magnitudes(ctx):
+    """f32 rows near both ends of the type whose products are ordinary."""
+    c = Cache(ctx, (4, 2, 128), "f32", [200])
+    g = torch.Generator("cuda").manual_seed(13)
+    for qs in (1e-35, 1e33):
+        c.rows = [(c.rows[0][0][:0], c.rows[0][1][:0])]
+        c.append([(c.random(200, g) / qs, c.random(200, g))])
+        q = c.queries(100, g) * qs
+        out, lse = c.prefill(q, [100])
+        ro, rl, to, tl = c.expect(0, q, range(100, 200))
+        near(out, ro, to, "prompt")
+        out, lse = c.decode(q[99:])
+        near(out, ro[99:], to[99:], "token")
+        near(lse, rl[99:], tl[99:], "lse")
 
 
 @pytest.mark.parametrize("dtype", TYPES)

@@ -380,6 +380,9 @@ int attention(vrt_ctx* ctx, const vrt_kv8_cache* cache, const vrt_kv8_attn* attn
     }
     if (!ctx) return fail(VRT_E_INVALID, "kv8: null context");
     if (count == 0) return VRT_OK;
+    if (static_cast<uint64_t>(max_new) / 16 * cache->kv_heads > 0x7fffffffull) {
+        return fail(VRT_E_UNSUPPORTED, "kv8 attention: max_new %u on %u KV heads exceeds a grid", max_new, cache->kv_heads);
+    }
     Kv8Attn p{};
     p.c = view_of(cache);
     p.q = d_q;

@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(kKdThreads, KdShape<HD>::kCtas) kv8_decode_ker
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 float& z = s[b >> 1][2 * (b & 1) + h];
-                z = z * ks * sc[h];
+                z = z * (ks * sc[h]);
                 if (plain_cap) z = capped<TERMS == 2>(z, p.a.softcap, inv_cap);
                 if (!see) z = -INFINITY;
                 top[h] = fmaxf(top[h], z);

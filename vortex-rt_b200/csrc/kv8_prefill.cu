@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(kKpThreads) kv8_prefill_kernel(const Kv8Split 
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 float& z = s[i][e];
-                z = z * k_now * sc[e >> 1];
+                z = z * (k_now * sc[e >> 1]);
                 if (cap) z = capped<TERMS == 2>(z, p.a.softcap, inv_cap);
                 if (!full) {
                     const int64_t t = t0 + 8 * i + 2 * t4 + (e & 1);
@@ -226,22 +226,17 @@ __global__ void __launch_bounds__(kKpThreads) kv8_prefill_kernel(const Kv8Split 
         uint32_t ph[2][4], pl[2][4];  // weights as the A operand of two k-steps of 16 keys
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            __half hi[4], lw[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float w = ex2(s[i][e] - m0[e >> 1]);
-                sum[e >> 1] += w;
+            for (int r = 0; r < 2; ++r) {  // this lane's two keys of row r
+                const float w0 = ex2(s[i][2 * r] - m0[r]), w1 = ex2(s[i][2 * r + 1] - m0[r]);
+                sum[r] += w0 + w1;
+                const __half2 hi = __floats2half2_rn(w0, w1);
+                ph[i >> 1][2 * (i & 1) + r] = *reinterpret_cast<const uint32_t*>(&hi);
                 if (TERMS == 2) {
-                    split_f16(w, hi[e], lw[e]);
-                } else {
-                    hi[e] = __float2half_rn(w);
+                    const float2 f = __half22float2(hi);
+                    const __half2 lw = __floats2half2_rn(w0 - f.x, w1 - f.y);
+                    pl[i >> 1][2 * (i & 1) + r] = *reinterpret_cast<const uint32_t*>(&lw);
                 }
-            }
-            ph[i >> 1][2 * (i & 1)] = pack_half(hi[0], hi[1]);
-            ph[i >> 1][2 * (i & 1) + 1] = pack_half(hi[2], hi[3]);
-            if (TERMS == 2) {
-                pl[i >> 1][2 * (i & 1)] = pack_half(lw[0], lw[1]);
-                pl[i >> 1][2 * (i & 1) + 1] = pack_half(lw[2], lw[3]);
             }
         }
         // a page that a row does not see adds nothing to it, even if its scale is NaN
