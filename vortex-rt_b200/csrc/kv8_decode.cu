@@ -205,6 +205,9 @@ __global__ void __launch_bounds__(kKdThreads, KdShape<HD>::kCtas) kv8_decode_ker
                     w[b][2] = u.z ^ 0x80808080u;
                     w[b][3] = u.w ^ 0x80808080u;
                 }
+                // f32 rows: each 64 dims on their own, joined by rounding additions
+                float part[2][4] = {};
+                float (&z)[2][4] = TERMS == 2 ? part : s;
 #pragma unroll
                 for (int st = 0; st < 4; ++st) {
                     const uint2 q0 = qf[(c * 4 + st) * 32 + lane];
@@ -214,9 +217,15 @@ __global__ void __launch_bounds__(kKdThreads, KdShape<HD>::kCtas) kv8_decode_ker
                     for (int m = 0; m < 2; ++m) {
                         const uint32_t a0 = codes_lo(w[2 * m][st]), a1 = codes_lo(w[2 * m + 1][st]);
                         const uint32_t a2 = codes_hi(w[2 * m][st]), a3 = codes_hi(w[2 * m + 1][st]);
-                        if (SETS == 2) mma_f16(s[m], a0, a1, a2, a3, q1);
-                        mma_f16(s[m], a0, a1, a2, a3, q0);
+                        if (SETS == 2) mma_f16(z[m], a0, a1, a2, a3, q1);
+                        mma_f16(z[m], a0, a1, a2, a3, q0);
                     }
+                }
+                if (TERMS == 2) {
+#pragma unroll
+                    for (int m = 0; m < 2; ++m)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[m][e] += part[m][e];
                 }
             }
         }

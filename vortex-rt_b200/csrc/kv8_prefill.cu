@@ -1,5 +1,7 @@
 // Prompt attention over the paged 8-bit KV cache (kv8.cuh): many query tokens
-// of each sequence at once, and the kernel that joins a split history.
+// of each sequence at once.  The form for f32 rows (and few rows of 64 dims),
+// the choice between it and the tcgen05 form (kv8_prefill_tc.cu), and the
+// kernels that join a split history.
 
 #include <cuda_runtime.h>
 
@@ -20,7 +22,13 @@ namespace vrt {
 // mma.sync m16n8k16 with fp32 sums.  As in the single-token kernel
 // (kv8_decode.cu) codes are exact, query rows and weights are fp16 or, for
 // f32 rows, fp16 + fp16 remainder, and a page's products start from zero and
-// join the fp32 sums by one FMA with the page's value scale.
+// join the fp32 sums by one FMA with the page's value scale.  tcgen05 sums in
+// TMEM and cuts them at every step, which f32 outputs of long histories would
+// show; its fp32 sums would have to leave TMEM for every key tile.
+// Bound by latency: f32 rows of 128 dims take 255 registers, so 8 warps an SM,
+// whose tensor pipe is active 37% of the time.  3x512 tokens behind histories
+// to 4096, window 1024 (32/16 heads of 128): 188 us.  Query fragments from
+// shared memory and 12 warps an SM took 201-221 us.
 constexpr int kKpRows = 64;
 constexpr int kKpThreads = 128;
 
@@ -166,8 +174,16 @@ __global__ void __launch_bounds__(kKpThreads) kv8_prefill_kernel(const Kv8Split 
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[i][e] = 0.0f;
         const __half* krow = ks + (lane % 8 + lane / 16 * 8) * Shape::kK + lane / 8 % 2 * 8;
+        float part[4][4];  // f32 rows: each 64 dims on their own, joined by rounding additions
+        float (&acc_s)[4][4] = TERMS == 2 ? part : s;
 #pragma unroll
         for (int st = 0; st < KS; ++st) {
+            if (TERMS == 2 && st % 4 == 0) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) part[i][e] = 0.0f;
+            }
             uint32_t b0[4], b1[4];  // keys 0-7 and 8-15, 16-23 and 24-31, both k halves
             ldmatrix4(b0, krow + 16 * st);
             ldmatrix4(b1, krow + 16 * Shape::kK + 16 * st);
@@ -180,10 +196,16 @@ __global__ void __launch_bounds__(kKpThreads) kv8_prefill_kernel(const Kv8Split 
                 } else {
                     ldmatrix4(a, qrow + t * kKpRows * Shape::kQ + 16 * st);
                 }
-                mma_f16(s[0], a[0], a[1], a[2], a[3], make_uint2(b0[0], b0[1]));
-                mma_f16(s[1], a[0], a[1], a[2], a[3], make_uint2(b0[2], b0[3]));
-                mma_f16(s[2], a[0], a[1], a[2], a[3], make_uint2(b1[0], b1[1]));
-                mma_f16(s[3], a[0], a[1], a[2], a[3], make_uint2(b1[2], b1[3]));
+                mma_f16(acc_s[0], a[0], a[1], a[2], a[3], make_uint2(b0[0], b0[1]));
+                mma_f16(acc_s[1], a[0], a[1], a[2], a[3], make_uint2(b0[2], b0[3]));
+                mma_f16(acc_s[2], a[0], a[1], a[2], a[3], make_uint2(b1[0], b1[1]));
+                mma_f16(acc_s[3], a[0], a[1], a[2], a[3], make_uint2(b1[2], b1[3]));
+            }
+            if (TERMS == 2 && st % 4 == 3) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[i][e] += part[i][e];
             }
         }
         // softmax: s[i][e] is row e / 2, key 8 i + 2 t4 + e % 2
@@ -297,27 +319,76 @@ __global__ void __launch_bounds__(kKpThreads) kv8_prefill_kernel(const Kv8Split 
 
 // -------------------------------------------------------------------- join
 
-constexpr int kKjThreads = 256;
+constexpr int kKjThreads = 256, kKjWarps = kKjThreads / 32;
+constexpr uint32_t kKjFew = 8;  // splits that one warp joins
 
-// CTA (head, query token, sequence): the splits' outputs in split order, 8
-// warps over the splits, then over each other.
+// Splits of query token i of sequence `seq` (0: the row does not exist), and
+// its row among the call's.
+__device__ __forceinline__ uint32_t kv8_row_splits(const Kv8Split& p, uint32_t seq, uint32_t i, uint64_t& row) {
+    int64_t r0;
+    const uint32_t rows = kv8_rows(p.a.cu, seq, p.a.max_new, p.a.status, r0);
+    if (i >= rows) return 0;
+    row = static_cast<uint64_t>(r0 + i);
+    const uint32_t i0 = i / p.tile * p.tile, i1 = min(rows, i0 + p.tile) - 1;
+    return kv8_used(kv8_span(p.a, seq, rows, i0, i1).count(), p.chunk);
+}
+
+// Up to kKjFew splits: a warp for each (query token, head), the splits' loads
+// in flight together; CTA (token group, sequence) of 8 warps.  One CTA a row
+// took 60 us for 8x128 tokens of 32 heads in two splits.
+template <typename T, int HD>
+__global__ void __launch_bounds__(kKjThreads) kv8_join_few_kernel(const Kv8Split p) {
+    const uint32_t at = blockIdx.x * kKjWarps + threadIdx.x / 32, i = at / p.a.H, h = at % p.a.H, seq = blockIdx.y;
+    const int lane = threadIdx.x % 32;
+    pdl_wait();
+    if (i >= p.a.max_new) return;
+    uint64_t row = 0;
+    const uint32_t used = kv8_row_splits(p, seq, i, row);
+    if (used <= 1) return;  // the only split wrote the output itself
+    const uint64_t first = ((static_cast<uint64_t>(seq) * p.a.max_new + i) * p.a.H + h) * p.splits;
+    const float* ml = p.part_ml + first * 2;
+    const float* part = p.part + first * HD;
+    float m = -INFINITY, l = 0.0f, f[kKjFew], v[HD / 32];
+#pragma unroll
+    for (uint32_t s = 0; s < kKjFew; ++s) m = s < used ? fmaxf(m, ml[2 * s]) : m;
+#pragma unroll
+    for (uint32_t s = 0; s < kKjFew; ++s) {
+        const bool there = s < used;
+        const float ms = there ? ml[2 * s] : -INFINITY;
+        f[s] = ms == -INFINITY ? 1.0f : ex2(ms - m);
+        l += there ? ml[2 * s + 1] * f[s] : 0.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < HD / 32; ++e) v[e] = 0.0f;
+#pragma unroll
+    for (uint32_t s = 0; s < kKjFew; ++s) {
+        if (s < used) {
+#pragma unroll
+            for (int e = 0; e < HD / 32; ++e) v[e] = fmaf(part[s * HD + lane + 32 * e], f[s], v[e]);
+        }
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    T* out = static_cast<T*>(p.a.out) + row * p.a.out_stride + static_cast<uint64_t>(h) * HD;
+#pragma unroll
+    for (int e = 0; e < HD / 32; ++e) out[lane + 32 * e] = from_f32<T>(v[e] * inv);
+    if (p.a.lse && lane == 0) p.a.lse[row * p.a.H + h] = kv8_lse(m, l);
+}
+
+// More splits: CTA (head, query token, sequence), 8 warps over the splits, in
+// split order, then over each other.
 template <typename T, int HD>
 __global__ void __launch_bounds__(kKjThreads) kv8_join_kernel(const Kv8Split p) {
-    constexpr int W = kKjThreads / 32;
     __shared__ float f[kKv8MaxSplits];
-    __shared__ float o[W][HD];
+    __shared__ float o[kKjWarps][HD];
     __shared__ float total;
     const uint32_t h = blockIdx.x, i = blockIdx.y, seq = blockIdx.z;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     pdl_wait();
-    int64_t r0;
-    const uint32_t rows = kv8_rows(p.a.cu, seq, p.a.max_new, p.a.status, r0);
-    if (i >= rows) return;
-    const uint32_t i0 = i / p.tile * p.tile, i1 = min(rows, i0 + p.tile) - 1;
-    const uint32_t used = kv8_used(kv8_span(p.a, seq, rows, i0, i1).count(), p.chunk);
-    if (used == 1) return;  // the only split wrote the output itself
-    const uint64_t at = (static_cast<uint64_t>(seq) * p.a.max_new + i) * p.a.H + h, row = static_cast<uint64_t>(r0 + i);
-    const float* ml = p.part_ml + at * p.splits * 2;
+    uint64_t row = 0;
+    const uint32_t used = kv8_row_splits(p, seq, i, row);
+    if (used <= 1) return;
+    const uint64_t first = ((static_cast<uint64_t>(seq) * p.a.max_new + i) * p.a.H + h) * p.splits;
+    const float* ml = p.part_ml + first * 2;
     if (warp == 0) {
         float m = -INFINITY, l = 0.0f;
         for (uint32_t s = lane; s < used; s += 32) m = fmaxf(m, ml[2 * s]);
@@ -334,12 +405,12 @@ __global__ void __launch_bounds__(kKjThreads) kv8_join_kernel(const Kv8Split p) 
         }
     }
     __syncthreads();
-    const float* part = p.part + at * p.splits * HD;
+    const float* part = p.part + first * HD;
     float v[HD / 32];
 #pragma unroll
     for (int e = 0; e < HD / 32; ++e) v[e] = 0.0f;
 #pragma unroll 4
-    for (uint32_t s = warp; s < used; s += W) {
+    for (uint32_t s = warp; s < used; s += kKjWarps) {
 #pragma unroll
         for (int e = 0; e < HD / 32; ++e) v[e] = fmaf(part[static_cast<uint64_t>(s) * HD + lane + 32 * e], f[s], v[e]);
     }
@@ -351,7 +422,7 @@ __global__ void __launch_bounds__(kKjThreads) kv8_join_kernel(const Kv8Split p) 
     for (int d = threadIdx.x; d < HD; d += kKjThreads) {
         float x = 0.0f;
 #pragma unroll
-        for (int w = 0; w < W; ++w) x += o[w][d];
+        for (int w = 0; w < kKjWarps; ++w) x += o[w][d];
         out[d] = from_f32<T>(x * inv);
     }
 }
@@ -359,9 +430,12 @@ __global__ void __launch_bounds__(kKjThreads) kv8_join_kernel(const Kv8Split p) 
 // -------------------------------------------------------------------- host
 
 cudaError_t kv8_join(const Kv8Split& p, uint32_t hd, int dtype, cudaStream_t s) {
-    const dim3 grid(p.a.H, p.a.max_new, p.a.count);
-#define VRT_KJ(TY, T, HD) \
-    if (dtype == TY && hd == HD) return launch(kv8_join_kernel<T, HD>, grid, dim3(kKjThreads), 0, s, true, p);
+    const bool few = p.splits <= kKjFew;
+    const uint64_t rows = static_cast<uint64_t>(p.a.max_new) * p.a.H;
+    const dim3 grid = few ? dim3(static_cast<uint32_t>((rows + kKjWarps - 1) / kKjWarps), p.a.count) : dim3(p.a.H, p.a.max_new, p.a.count);
+#define VRT_KJ(TY, T, HD)                                                                                             \
+    if (dtype == TY && hd == HD)                                                                                      \
+        return launch(few ? kv8_join_few_kernel<T, HD> : kv8_join_kernel<T, HD>, grid, dim3(kKjThreads), 0, s, true, p);
 #define VRT_KJ3(HD) VRT_KJ(VRT_F32, float, HD) VRT_KJ(VRT_F16, __half, HD) VRT_KJ(VRT_BF16, __nv_bfloat16, HD)
     VRT_KJ3(64) VRT_KJ3(128) VRT_KJ3(256)
 #undef VRT_KJ3
@@ -369,28 +443,34 @@ cudaError_t kv8_join(const Kv8Split& p, uint32_t hd, int dtype, cudaStream_t s) 
     return cudaErrorInvalidValue;
 }
 
-// Splits of a history when there are too few query tiles for the GPU: about
-// two CTAs an SM, kKpMinPages pages each at least.
-constexpr uint32_t kKpMinPages = 8;
-
 // Query tokens of a CTA, and whether the tcgen05 form runs: for 16-bit rows,
-// when a sequence may bring more rows than one tile of the warp form has.
+// always from head_dim 128 up, at head_dim 64 from 512 rows a sequence.
+// Measured, tcgen05 and warp form (bf16, us): 32/16 heads of 128, 2 tokens
+// behind 8192 31.9 and 34.7, 64 tokens 43.6 and 67.2, 1024 tokens 190 and 848;
+// 4/1 heads of 256, 2 tokens behind 1024 23.5 and 34.3; 8/2 heads of 64, 32
+// tokens behind 1024 16.1 and 14.1, 64 behind 8192 20.9 and 18.4, 128 behind
+// 8192 21.5 and 28.2.
 static bool kp_tile(uint32_t hd, int dtype, uint32_t group, uint32_t max_new, uint32_t& tile) {
-    const bool tc = dtype != VRT_F32 && static_cast<uint64_t>(max_new) * group > kKpRows;
+    const bool tc = dtype != VRT_F32 && (hd >= 128 || static_cast<uint64_t>(max_new) * group >= 512);
     tile = tc ? kv8_prefill_tc_rows(hd) / 128 * (128 / group) : kKpRows / group;
     return tc;
 }
 
-static uint64_t kp_cap(int sms, uint32_t tile, uint32_t kv, uint32_t count, uint32_t max_new) {
+// Splits of a history when there are too few query tiles for the GPU: up to
+// two CTAs an SM of the warp form, one of the tcgen05 form, kKpMinPages pages
+// each at least.
+constexpr uint32_t kKpMinPages = 8;
+
+static uint64_t kp_cap(int sms, bool tc, uint32_t tile, uint32_t kv, uint32_t count, uint32_t max_new) {
     const uint64_t ctas = (static_cast<uint64_t>(max_new) + tile - 1) / tile * kv * std::max(1u, count);
-    const uint64_t want = std::min<uint64_t>(2ull * sms / std::max<uint64_t>(1, ctas), kKv8MaxSplits);
+    const uint64_t want = std::min<uint64_t>((tc ? 1ull : 2ull) * sms / std::max<uint64_t>(1, ctas), kKv8MaxSplits);
     return max_new > 65535u ? 1 : std::max<uint64_t>(1, std::min<uint64_t>(want, 65535u / std::max(1u, count)));  // grid limits
 }
 
 static bool kp_plan(int sms, uint32_t hd, const Kv8Attn& a, uint32_t& tile, uint32_t& chunk, uint32_t& splits) {
     const bool tc = kp_tile(hd, a.dtype, a.H / a.c.kv, a.max_new, tile);
     const uint64_t pages = (static_cast<uint64_t>(a.max_len) + kKv8Page - 1) / kKv8Page;
-    const uint64_t cap = kp_cap(sms, tile, a.c.kv, a.count, a.max_new);
+    const uint64_t cap = kp_cap(sms, tc, tile, a.c.kv, a.count, a.max_new);
     const uint64_t c = std::max<uint64_t>((pages + cap - 1) / cap, kKpMinPages);
     chunk = static_cast<uint32_t>(c);
     splits = static_cast<uint32_t>((pages + c - 1) / c);
@@ -401,9 +481,9 @@ static bool kp_plan(int sms, uint32_t hd, const Kv8Attn& a, uint32_t& tile, uint
 uint64_t kv8_prefill_workspace(int sms, uint32_t hd, int dtype, uint32_t kv, uint32_t heads, uint32_t count,
                                uint32_t max_new, uint32_t max_len) {
     uint32_t tile;
-    kp_tile(hd, dtype, heads / kv, max_new, tile);
+    const bool tc = kp_tile(hd, dtype, heads / kv, max_new, tile);
     const uint64_t pages = (static_cast<uint64_t>(max_len) + kKv8Page - 1) / kKv8Page;
-    const uint64_t splits = std::min<uint64_t>(kp_cap(sms, tile, kv, count, max_new),
+    const uint64_t splits = std::min<uint64_t>(kp_cap(sms, tc, tile, kv, count, max_new),
                                                (pages + kKpMinPages - 1) / kKpMinPages);
     return splits > 1 ? static_cast<uint64_t>(count) * max_new * heads * splits * (hd + 2) * 4 : 0;
 }
@@ -438,14 +518,13 @@ cudaError_t kv8_prefill(const Kv8Attn& a, uint32_t hd, int sms, void* workspace,
     p.part = static_cast<float*>(workspace);
     p.part_ml = p.part + static_cast<uint64_t>(a.count) * a.max_new * a.H * p.splits * hd;
     if (tc) return kv8_prefill_tc(p, hd, s);
-#define VRT_KP(HD)                                                                \
-    if (hd == HD) {                                                               \
-        if (a.dtype == VRT_F16) return kp_launch<__half, HD, 1>(p, s);            \
-        if (a.dtype == VRT_BF16) return kp_launch<__nv_bfloat16, HD, 1>(p, s);    \
-        return kp_launch<float, HD, 2>(p, s);                                     \
+    if (a.dtype == VRT_F32) {
+        if (hd == 64) return kp_launch<float, 64, 2>(p, s);
+        if (hd == 128) return kp_launch<float, 128, 2>(p, s);
+        if (hd == 256) return kp_launch<float, 256, 2>(p, s);
+    } else if (hd == 64) {
+        return a.dtype == VRT_F16 ? kp_launch<__half, 64, 1>(p, s) : kp_launch<__nv_bfloat16, 64, 1>(p, s);
     }
-    VRT_KP(64) VRT_KP(128) VRT_KP(256)
-#undef VRT_KP
     return cudaErrorInvalidValue;
 }
 
