@@ -270,7 +270,12 @@ typedef struct {
 /* Append rows [d_cu[i], d_cu[i+1]) of d_k / d_v ([rows][kv_heads][head_dim],
  * consecutive rows row_stride elements apart; 0 = packed) to sequence i, which
  * holds d_start[i] tokens, for i < count.  d_cu NULL: one row each.  max_new:
- * the most rows of one sequence.  Rows must start on 16-byte boundaries. */
+ * the most rows of one sequence.  Rows must start on 16-byte boundaries.
+ * A sequence may be taken back to fewer tokens (start below what it holds) as
+ * far as its tail reaches: within its last page if that is not full, or to any
+ * multiple of VRT_KV8_PAGE.  Likewise it may start on pages shared with
+ * another sequence at a multiple of VRT_KV8_PAGE, or else with a copy of that
+ * one's last page and tail. */
 VRT_API int vrt_kv8_append(vrt_ctx* ctx, const vrt_kv8_cache* cache, const void* d_k, const void* d_v,
                            uint64_t row_stride, const int32_t* d_start, const int32_t* d_cu, uint32_t count,
                            uint32_t max_new, void* stream);

@@ -454,12 +454,13 @@ def test_non_finite_in_sight(ctx, dtype, which):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("cap", [0.0, 30.0])
 @pytest.mark.parametrize("window", [0, 1, 2])
-def test_nan_query(ctx, dtype, cap, window):
-    """A NaN in a query gives NaN in its own token and head alone, whatever the key that it sees."""
-    c = Cache(ctx, (8, 2, 64), dtype, [130])
+@pytest.mark.parametrize("heads,value", [((8, 2, 64), math.nan), ((8, 2, 128), math.nan), ((8, 2, 64), math.inf), ((8, 2, 128), -math.inf)])
+def test_non_finite_query(ctx, dtype, cap, window, heads, value):
+    """A NaN or an infinity in a query gives NaN in its own token and head alone, whatever the key that it sees."""
+    c = Cache(ctx, heads, dtype, [130])
     g = fill(c, [130])
     q = c.queries(130, g)
-    q[17, 3, 5] = q[38, 0, 63] = q[127, 7, 0] = math.nan
+    q[17, 3, 5] = q[38, 0, 63] = q[127, 7, 0] = value
     bad = torch.zeros((130, 8), dtype=torch.bool, device="cuda")
     bad[17, 3] = bad[38, 0] = bad[127, 7] = True
     out, lse = c.prefill(q, [130], window=window, cap=cap)
@@ -467,6 +468,49 @@ def test_nan_query(ctx, dtype, cap, window):
     assert torch.equal(torch.isnan(lse), bad)
     out, lse = c.decode(q[127:128], window=window, cap=cap)
     assert torch.equal(torch.isnan(out).all(2), bad[127:128]) and torch.equal(torch.isnan(out).any(2), bad[127:128])
+
+
+@pytest.mark.parametrize("heads,dtype", [((8, 2, 128), "bf16"), ((4, 1, 256), "f16"), ((8, 1, 64), "bf16"), ((4, 2, 128), "f32")])
+def test_prompt_without_a_page(ctx, heads, dtype):
+    """A page that is not in the pool is left out of a prompt's attention; an upper bound of rows far above the rows."""
+    c = Cache(ctx, heads, dtype, [600, 600])
+    g = fill(c, [500, 450])
+    q = c.queries(500, g)
+    good, _ = c.prefill(q, [300, 200], max_new=600)
+    assert status(ctx) == 0
+    c.table[0, 5] = c.pages + 7
+    out, lse = c.prefill(q, [300, 200], max_new=600)
+    assert status(ctx) == 32
+    assert torch.equal(out[300:], good[300:])
+    r = c.h // c.kv
+    k, v = c.values(0)
+    keep = torch.ones(500, dtype=torch.bool, device="cuda")
+    keep[160:192] = False
+    t = torch.arange(500, device="cuda")
+    see = keep & (t <= torch.arange(200, 500, device="cuda")[:, None])
+    s = torch.einsum("mhd,thd->mht", q[:300].double(), k.repeat_interleave(r, 1)) * c.hd ** -0.5
+    s = torch.where(see[:, None], s, -math.inf)
+    ref = torch.einsum("mht,thd->mhd", torch.softmax(s, 2), v.repeat_interleave(r, 1))
+    _, _, tol, tl = c.expect(0, q[:300], range(200, 500))
+    # the weights' sum is smaller by what the page had: tolerances grow with it
+    grow = torch.exp(torch.logsumexp(torch.einsum("mhd,thd->mht", q[:300].double(), k.repeat_interleave(r, 1)) * c.hd ** -0.5
+                                     + torch.where((t <= torch.arange(200, 500, device="cuda")[:, None])[:, None], 0.0, -math.inf), 2)
+                     - torch.logsumexp(s, 2))
+    near(out[:300], ref, tol * grow[..., None] + HALF[dtype] * ref.abs(), "out")
+    near(lse[:300], torch.logsumexp(s, 2), tl, "lse")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_taken_back(ctx, dtype):
+    """A sequence taken back within its last page, and to a multiple of a page, then grown on."""
+    c = Cache(ctx, (4, 2, 64), dtype, [200])
+    g = fill(c, [110])
+    for keep in (100, 97, 96, 64):
+        c.rows = [(c.rows[0][0][:keep], c.rows[0][1][:keep])]
+        c.append([(c.random(20, g), c.random(20, g))])
+        (k, v), = c.read()
+        rk, rv = c.values(0)
+        assert torch.equal(k.double(), rk) and torch.equal(v.double(), rv), keep
 
 
 def test_out_of_range(ctx):

@@ -295,7 +295,7 @@ uint32_t type_size(int dtype) { return dtype == VRT_F32 ? 4u : 2u; }
 
 uint32_t* status_word(vrt_ctx* ctx) { return reinterpret_cast<uint32_t*>(ctx->d_key) + 2; }
 
-int check_cache(const vrt_kv8_cache* c) {
+int check_shape(const vrt_kv8_cache* c) {
     if (!c) return fail(VRT_E_INVALID, "kv8: null argument");
     if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) {
         return fail(VRT_E_UNSUPPORTED, "kv8: head_dim %u is not 64, 128 or 256", c->head_dim);
@@ -307,6 +307,11 @@ int check_cache(const vrt_kv8_cache* c) {
     if (!c->pages_per_seq || c->pages_per_seq > 0x7fffffffu / kKv8Page) {
         return fail(VRT_E_INVALID, "kv8: pages_per_seq must be 1..%u", 0x7fffffffu / kKv8Page);
     }
+    return VRT_OK;
+}
+
+int check_cache(const vrt_kv8_cache* c) {
+    VRT_TRY(check_shape(c));
     const void* ptrs[] = {c->d_k, c->d_v, c->d_k_scale, c->d_v_scale, c->d_k_tail, c->d_v_tail, c->d_table};
     for (const void* p : ptrs) {
         if (!p) return fail(VRT_E_INVALID, "kv8: the cache lacks an array");
@@ -471,7 +476,7 @@ int vrt_kv8_read(vrt_ctx* ctx, const vrt_kv8_cache* cache, const int32_t* d_star
 int vrt_kv8_workspace(vrt_ctx* ctx, const vrt_kv8_cache* cache, uint32_t heads, uint32_t count, uint32_t max_new,
                       uint32_t max_len, uint64_t* bytes) {
     clear_error();
-    VRT_TRY(check_cache(cache));
+    VRT_TRY(check_shape(cache));  // the arrays may come later
     if (!bytes) return fail(VRT_E_INVALID, "kv8 workspace: null argument");
     VRT_TRY(check_batch(cache, count, max_len, "max_len"));
     VRT_TRY(check_batch(cache, count, max_new, "max_new"));

@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(kKdThreads, KdShape<HD>::kCtas) kv8_decode_ker
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         const float mul = kv8_row_unit(m);
-        if (piece == 0) q_unit[h] = 1.0f / mul;
+        if (piece == 0) q_unit[h] = m < INFINITY ? 1.0f / mul : NAN;  // an infinity makes the row NaN, capped or not
         __half* f = reinterpret_cast<__half*>(qf);
 #pragma unroll
         for (int e = 0; e < E; ++e) {

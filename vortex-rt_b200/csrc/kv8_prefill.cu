@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(kKpThreads) kv8_prefill_kernel(const Kv8Split 
         }
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
         const float mul = kv8_row_unit(m);
-        if (half == 0) unit[r] = 1.0f / mul;
+        if (half == 0) unit[r] = m < INFINITY ? 1.0f / mul : NAN;  // an infinity makes the row NaN, capped or not
         for (int d = 0; d < HD / 2; d += 8) {
             float x[8];
             load_row<T, 8>(q + d, x);
