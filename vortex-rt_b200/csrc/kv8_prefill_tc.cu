@@ -193,6 +193,20 @@ __device__ __forceinline__ uint32_t pack_rows<__nv_bfloat16>(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// The largest magnitude of eight 16-bit values, as bits (ordered like the
+// values), and what it stands for.
+template <typename T>
+__device__ __forceinline__ uint32_t row_top(const uint4& u) {
+    const uint32_t w[4] = {u.x & 0x7fff7fffu, u.y & 0x7fff7fffu, u.z & 0x7fff7fffu, u.w & 0x7fff7fffu};
+    const uint32_t m = __vmaxu2(__vmaxu2(w[0], w[1]), __vmaxu2(w[2], w[3]));
+    return max(m & 0xffffu, m >> 16);
+}
+template <typename T>
+__device__ __forceinline__ float row_magnitude(uint32_t top) {
+    const unsigned short bits = static_cast<unsigned short>(top);
+    return to_f32(*reinterpret_cast<const T*>(&bits));
+}
+
 // 16 codes as fp16 into two 16-byte pieces of a swizzled tile row.
 __device__ __forceinline__ void store_codes(uint8_t* a, uint8_t* b, uint4 u) {
     const uint32_t w[4] = {u.x ^ 0x80808080u, u.y ^ 0x80808080u, u.z ^ 0x80808080u, u.w ^ 0x80808080u};
@@ -318,29 +332,27 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
         float unit = 0.0f;  // score units of a row
         {
             const T* q = static_cast<const T*>(p.a.q) + at * p.a.q_stride + static_cast<uint64_t>(live ? h : g * R) * HD;
-            float m = 0.0f;
-            bool finite = true;
-#pragma unroll 2
-            for (int d = 0; d < HD; d += 8) {
-                float x[8];
-                load_row<T, 8>(q + d, x);
-                m = fmaxf(m, max_abs(x));
+            // the whole row on its way at once: its latency is the CTA's start
+            uint4 raw[HD / 8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) finite = finite && fabsf(x[e]) < INFINITY;
-            }
+            for (int d = 0; d < HD / 8; ++d) raw[d] = reinterpret_cast<const uint4*>(q)[d];
+            uint32_t top = 0;  // of the magnitudes' bits: infinities and NaN above all numbers
+#pragma unroll
+            for (int d = 0; d < HD / 8; ++d) top = max(top, row_top<T>(raw[d]));
+            const float m = row_magnitude<T>(top);
+            const bool finite = m < INFINITY;
             const float mul = kv8_row_unit(m);
             unit = finite ? 1.0f / mul * fabsf(p.a.scale) : NAN;
             const float sign = live ? (p.a.scale < 0.0f ? -mul : mul) : 0.0f;
-#pragma unroll 2
-            for (int d = 0; d < HD; d += 8) {
-                float x[8];
-                load_row<T, 8>(q + d, x);
+#pragma unroll
+            for (int d = 0; d < HD / 8; ++d) {
+                const T* x = reinterpret_cast<const T*>(&raw[d]);
                 uint32_t w[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    w[e] = live ? pack_half(__float2half_rn(x[2 * e] * sign), __float2half_rn(x[2 * e + 1] * sign)) : 0u;
+                    w[e] = live ? pack_half(__float2half_rn(to_f32(x[2 * e]) * sign), __float2half_rn(to_f32(x[2 * e + 1]) * sign)) : 0u;
                 }
-                *reinterpret_cast<uint4*>(sq + t * Shape::kQTile + d / 64 * (128 * 128) + sw128_offset(row, d % 64)) =
+                *reinterpret_cast<uint4*>(sq + t * Shape::kQTile + d / 8 * (128 * 128) + sw128_offset(row, d % 8 * 8)) =
                     make_uint4(w[0], w[1], w[2], w[3]);
             }
             fence_proxy_async_smem();
@@ -494,7 +506,7 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
         const float mul = used == 1 ? (sum == 0.0f ? 0.0f : ref / sum) : ref;
         T* out = static_cast<T*>(p.a.out) + at * p.a.out_stride + static_cast<uint64_t>(h) * HD;
         const uint64_t prow = ((static_cast<uint64_t>(seq) * p.a.max_new + i0 + token) * p.a.H + h) * p.splits + split;
-#pragma unroll 1
+#pragma unroll 2
         for (int d = 0; d < HD; d += 16) {
             uint32_t v[16] = {};
             if (mine > 0) tmem_ld16(tmem + lanes + Shape::kOCol + t * HD + d, v);
@@ -531,22 +543,6 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
         constexpr int C = PG * HD * 2 / 128;  // 16-byte pieces of a block that a thread brings
         constexpr int kPieces = HD * 2 / 128; // of them in a page
         float ref = 1.0f;
-        if (keys) {
-            // the largest value scale among the CTA's pages
-            float m = 0.0f;
-            for (uint32_t i = j0 + c0; i < j1; i += 128) {
-                const int id = kv8_page(p.a.c, seq, span.page(i), p.a.status);
-                const float s = id < 0 ? 0.0f : p.a.c.v_scale[static_cast<uint64_t>(id) * p.a.c.kv + g];
-                if (s < INFINITY) m = fmaxf(m, s);
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            if (lane == 0) reference[warp - 4 * MT] = m;
-            named_bar_sync(1, 128);
-            m = fmaxf(fmaxf(reference[0], reference[1]), fmaxf(reference[2], reference[3]));
-            if (m > 0.0f) ref = m;
-            if (c0 == 0) reference[4] = ref;
-        }
         // Piece i of a thread is 128 pieces behind piece i - 1: a whole number of the periods below, so its page, its
         // offset in the page and in the operand tile are constants away.  Pieces are dealt so that a quarter warp's
         // stores meet all banks: 64 dims of two keys; 4 dims of values from both halves of a swizzle period.
@@ -629,6 +625,22 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
                 const uint64_t head = static_cast<uint64_t>(max(id, 0)) * p.a.c.kv + g;
                 ks = __ldg(p.a.c.k_scale + head);
                 vs = __ldg(p.a.c.v_scale + head);
+            }
+            if (keys && j == -1) {
+                // the largest value scale among the CTA's pages, while the first block's codes travel
+                float m = 0.0f;
+                for (uint32_t i = j0 + c0; i < j1; i += 128) {
+                    const int id = kv8_page(p.a.c, seq, span.page(i), p.a.status);
+                    const float v = id < 0 ? 0.0f : p.a.c.v_scale[static_cast<uint64_t>(id) * p.a.c.kv + g];
+                    if (v < INFINITY) m = fmaxf(m, v);
+                }
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                if (lane == 0) reference[warp - 4 * MT] = m;
+                named_bar_sync(1, 128);
+                m = fmaxf(fmaxf(reference[0], reference[1]), fmaxf(reference[2], reference[3]));
+                if (m > 0.0f) ref = m;
+                if (c0 == 0) reference[4] = ref;
             }
         }
     } else {
