@@ -561,7 +561,8 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
         for (int j = -2; j < blocks_k; ++j) {  // store block j, ask for block j + 1, look block j + 2 up
             if (j >= 0) {
                 const int s = j % ST;
-                if (j >= ST) ok = ok && mbar_wait_bounded(empty + s, ((j / ST) - 1) & 1);
+                // as one warp: lanes that gave up alone would leave the others in the warp barrier below
+                if (j >= ST) ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded(empty + s, ((j / ST) - 1) & 1));
                 if (!ok) break;
                 uint8_t* at = stages + s * Shape::kKTile;
                 if (keys) {
