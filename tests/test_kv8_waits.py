@@ -26,3 +26,17 @@ def test_prompt_kernel_votes():
     assert len(waits) >= 5
     for s in waits:
         assert "ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded(" in s or s == "mbar_wait_bounded(drained + t, 0)", s
+
+
+def test_token_kernel_ends():
+    """A wait of the single-token kernel that gives up, in any lane, is the last but for the copies under way: no page
+    behind it is waited for, a second each, and no copy is asked for into a slot whose last one may still land."""
+    text = source("kv8_decode.cu")
+    refill = text[text.index("auto refill"):]
+    refill = refill[:refill.index("};")]
+    assert "ok = __all_sync(0xffffffffu, ok)" in refill and "if (ok && issued < 2 * mine)" in refill
+    assert re.search(r"for \(uint32_t i = 0; i < mine && ok; \+\+i\)", text)
+    waits = statements(text, "mbar_wait_bounded(")
+    assert len(waits) == 3 and sum(s.startswith("ok &= ") for s in waits) == 2, waits
+    drain = text[text.index("if (!ok) {"):]
+    assert drain.index("mbar_wait_bounded") < drain.index("atomicOr") < drain.index("__syncthreads")

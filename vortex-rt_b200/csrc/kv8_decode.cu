@@ -167,13 +167,14 @@ __global__ void __launch_bounds__(kKdThreads, KdShape<HD>::kCtas) kv8_decode_ker
     float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
     bool ok = true;
     uint32_t used = 0;  // ring items consumed
-    auto refill = [&](uint32_t base) {
+    auto refill = [&](uint32_t base) {  // after a wait that gave up, in any lane: no more copies, and the page is the last
         ++used;
+        ok = __all_sync(0xffffffffu, ok);
         __syncwarp();
-        if (issued < 2 * mine) issue(base);
+        if (ok && issued < 2 * mine) issue(base);
     };
 
-    for (uint32_t i = 0; i < mine; ++i) {
+    for (uint32_t i = 0; i < mine && ok; ++i) {
         const uint32_t base = i & ~31u;
         if (i == base && i) {
             id_now = id_next;
@@ -319,7 +320,11 @@ __global__ void __launch_bounds__(kKdThreads, KdShape<HD>::kCtas) kv8_decode_ker
         }
         refill(base);
     }
-    if (!ok && lane == 0) atomicOr(p.a.status, kStatusWaitTimeout);
+    if (!ok) {
+        // the copies still under way, each slot's latest, land before their ring is used below
+        for (uint32_t i = issued > D ? issued - D : 0; i < issued; ++i) mbar_wait_bounded(bar + i % D, (i / D) & 1);
+        if (lane == 0) atomicOr(p.a.status, kStatusWaitTimeout);
+    }
 
     // ---- join the warps: [warp][column][HD] outputs over the rings, then maxima and sums
 #pragma unroll
