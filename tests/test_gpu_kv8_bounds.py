@@ -1,0 +1,97 @@
+"""Where 16-bit attention over the paged 8-bit KV cache can lose a result:
+scores far from 0.  Against plain implementations in 64 bits, as in
+test_gpu_kv8.py, with tolerances that depend on what a row sees alone."""
+
+import math
+
+import pytest
+
+from test_gpu_kv8 import HALF, I32, PAGE, TYPES, Cache, clean_status, near, status  # noqa: F401
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -23  # a step of fp32: what an addition that cuts loses at most
+FAST_CAP = 128.0  # up to here 16-bit rows take cap - 2 cap / (e^2y + 1)
+
+
+def exact(c, i, q, pos, window=0, prefix=0, cap=0.0, tc=False):
+    """q [m, h, hd] of positions pos -> out, lse and their tolerances, in 64 bits.
+
+    A score is a sum of hd products in fp32: each addition may be cut, a step U of the sum of magnitudes; eight more
+    for its factors.  tanh does not widen that, and adds: up to a cap of FAST_CAP the difference of two numbers of the
+    cap's size, each off by a step or two (4 U cap); above it eight steps of the score itself.  A weight is off by
+    twice the largest score error of its row, and in the 16-bit types by half an fp16 step (2^-11); the capped prompt
+    form's polynomial adds 2^-18.  A weight's fp16 form ends at 2^-39 of the largest weight (2^14 times it are held,
+    and fp16's last half step is 2^-25), in the tcgen05 form (`tc`) at 2^-28 (the largest is held at 2^3 at least).
+    Sums: a product of 16 keys is one addition to fp32 that may be cut, in runs of at most 16,384 keys; pages, and
+    such runs, are joined by rounding additions.  The stored value is off by half a step of its type."""
+    k, v = c.values(i)
+    n, (m, h, hd) = k.shape[0], q.shape
+    r = h // c.kv
+    kk, vv = k.repeat_interleave(r, 1), v.repeat_interleave(r, 1)
+    s = torch.einsum("mhd,thd->mht", q.double(), kk) * hd ** -0.5
+    mag = torch.einsum("mhd,thd->mht", q.double().abs(), kk.abs()) * hd ** -0.5
+    if cap:
+        s = cap * torch.tanh(s / cap)
+    t = torch.arange(n, device="cuda")
+    p = torch.as_tensor(list(pos), device="cuda")[:, None]
+    see = (t < prefix) | ((t <= p) & ((p - t < window) if window else (t >= 0)))
+    s = torch.where(see[:, None], s, -math.inf)
+    ds = (hd + 8) * U * torch.where(see[:, None], mag, 0.0).amax(2)
+    if cap:
+        ds = ds + (4 * cap * U if cap <= FAST_CAP else 8 * U * torch.where(see[:, None], s.abs(), 0.0).amax(2))
+    lse = torch.logsumexp(s, 2)
+    w = torch.exp(s - torch.where(torch.isfinite(lse), lse, 0.0)[..., None])
+    # a value that nobody of the call sees may be anything
+    vz = torch.where(see.any(0)[:, None, None], vv, 0.0)
+    out = torch.einsum("mht,thd->mhd", w, vz)
+    amount = torch.einsum("mht,thd->mhd", w, vz.abs())
+    sums = (min(n, 16384) / 16 + n / PAGE + 16) * U
+    weight = 0.0 if c.dtype == "f32" else 2.0 ** -11 + (2.0 ** -17 if cap and tc else 0.0)
+    fi = torch.finfo(TYPES[c.dtype])
+    tol = HALF[c.dtype] * out.abs() + fi.tiny * fi.eps / 2 + amount * (2 * ds + sums + weight)[..., None]
+    cut = torch.einsum("mt,thd->mhd", see.double(), vz.abs()) * w.amax(2)[..., None]
+    tol = tol + (2.0 ** -28 if tc else 2.0 ** -39) * cut
+    return out, lse, tol, ds + sums + lse.abs().nan_to_num(0, 0, 0) * U
+
+
+def uses_tc(c, new):
+    """The prompt form of these sizes (16-bit rows from head_dim 128 up, or 512 rows of 64)."""
+    return c.dtype != "f32" and (c.hd >= 128 or new * c.h // c.kv >= 512)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads", [(8, 2, 64), (8, 2, 128), (4, 1, 256)])
+@pytest.mark.parametrize("far", [2.0 ** 19, 2.0 ** 22, 2.0 ** 24, 2.0 ** 25, 2.0 ** 26, 2.0 ** 27, 2.0 ** 28, 1e12, 1e30])
+def test_huge_scores(ctx, heads, dtype, far):
+    """Finite scores whose fp32 steps are whole numbers: each row is its highest key's value.
+
+    All queries lie along one direction, one key does so at full length: its score leads by half its size or more,
+    so every other weight is 0 in any precision."""
+    if dtype == "f16" and far > 1e10:
+        return  # out of the type's reach
+    n, m = 300, 150
+    c = Cache(ctx, heads, dtype, [n])
+    g = torch.Generator("cuda").manual_seed(22)
+    u = torch.where(torch.rand((c.hd,), generator=g, device="cuda") < 0.5, -1.0, 1.0)
+    length = math.sqrt(far / math.sqrt(c.hd))  # of a query, and of the key: score = length^2 sqrt(hd)
+    k, v = c.random(n, g).float().clamp(-4, 4) * (length / 64), c.random(n, g)
+    k[33] = length * u
+    c.append([(k.to(TYPES[dtype]), v)])
+    q = (length * u * torch.linspace(0.6, 2.1, m * c.h, device="cuda").view(m, c.h, 1)).to(TYPES[dtype])
+    want = c.values(0)[1][33].repeat_interleave(c.h // c.kv, 0)
+    # the one weight is an fp16 operand in the 16-bit types (half a step, 2^-11), its sum is not; then a product by the
+    # page's scale, a reciprocal and its product, a step each, and the stored value
+    tol = want.abs() * (HALF[dtype] + (0.0 if dtype == "f32" else 2.0 ** -11) + 4 * U) + 2.0 ** -25
+    for rows in (slice(0, m), slice(m - 20, m)):
+        out, lse = c.prefill(q[rows], [rows.stop - rows.start])
+        near(out, want.expand(out.shape), tol.expand(out.shape), "prompt")
+        assert torch.isfinite(lse).all()
+    for row in range(0, m, 7):
+        out, lse = c.decode(q[row:row + 1])
+        near(out, want[None], tol[None], "token")
+        assert torch.isfinite(lse).all()
+    # lse: the score, whose products' sum may be cut at each of hd additions
+    top = torch.einsum("mhd,hd->mh", q[-1:].double(), c.values(0)[0][33].repeat_interleave(c.h // c.kv, 0)) * c.hd ** -0.5
+    near(lse if row == m - 1 else c.decode(q[-1:])[1], top, (c.hd + 24) * U * top.abs(), "lse")

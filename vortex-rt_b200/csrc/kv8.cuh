@@ -170,6 +170,14 @@ __device__ __forceinline__ uint32_t kv8_share(uint32_t n, uint32_t used) { retur
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kKv8Lift = 14.0f;  // weights are held times 2^14
 
+// What a row of maximum mx weighs its scores from (base 2): the lift below it.
+// From 2^24 up a step of fp32 is 2 and more, and the lift could round up to 16,
+// past fp16: then from the maximum itself.
+__device__ __forceinline__ float kv8_base(float mx) {
+    const float m = mx - kKv8Lift;
+    return mx - m > 15.0f ? mx : m;
+}
+
 // ln of a sum l of weights 2^(z - m): nothing seen -> -inf, NaN stays.
 __device__ __forceinline__ float kv8_lse(float m, float l) {
     return l == 0.0f ? -INFINITY : (m == -INFINITY ? l : m / kLog2e + logf(l));

@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(kKdThreads, KdShape<HD>::kCtas) kv8_decode_ker
     for (int i = 0; i < KS; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[i][e] = 0.0f;
-    float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+    float mx[2] = {-INFINITY, -INFINITY}, m0[2] = {0.0f, 0.0f}, sum[2] = {0.0f, 0.0f};  // m0: what scores are weighed from
     bool ok = true;
     uint32_t used = 0;  // ring items consumed
     auto refill = [&](uint32_t base) {  // after a wait that gave up, in any lane: no more copies, and the page is the last
@@ -265,13 +265,13 @@ __global__ void __launch_bounds__(kKdThreads, KdShape<HD>::kCtas) kv8_decode_ker
                 f[h] = mx[h] == -INFINITY ? 0.0f : ex2(mx[h] - top[h]);
                 sum[h] *= f[h];
                 mx[h] = top[h];
+                m0[h] = mx[h] == -INFINITY ? 0.0f : kv8_base(mx[h]);
             }
 #pragma unroll
             for (int q = 0; q < KS; ++q)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[q][e] *= f[e & 1];
         }
-        const float m0[2] = {mx[0] == -INFINITY ? 0.0f : mx[0] - kKv8Lift, mx[1] == -INFINITY ? 0.0f : mx[1] - kKv8Lift};
         uint32_t ph[4], pl[4];
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(kKdThreads, KdShape<HD>::kCtas) kv8_decode_ker
     if (g8 == 0 && (!kPacked || t4 < 2)) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            wm[(warp * 8 + 2 * t4 + h) * 2] = mx[h] - kKv8Lift;  // sums are times 2^14
+            wm[(warp * 8 + 2 * t4 + h) * 2] = kv8_base(mx[h]);  // as the sums are weighed
             wm[(warp * 8 + 2 * t4 + h) * 2 + 1] = sum[h];
         }
     }

@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(kKpThreads) kv8_prefill_kernel(const Kv8Split 
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[i][e] *= f[e >> 1];
         }
-        const float m0[2] = {mx[0] == -INFINITY ? 0.0f : mx[0] - kKv8Lift, mx[1] == -INFINITY ? 0.0f : mx[1] - kKv8Lift};
+        const float m0[2] = {mx[0] == -INFINITY ? 0.0f : kv8_base(mx[0]), mx[1] == -INFINITY ? 0.0f : kv8_base(mx[1])};
         uint32_t ph[2][4], pl[2][4];  // weights as the A operand of two k-steps of 16 keys
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(kKpThreads) kv8_prefill_kernel(const Kv8Split 
                 out[8 * d + 2 * t4] = from_f32<T>(acc[d][2 * i] * inv);
                 out[8 * d + 2 * t4 + 1] = from_f32<T>(acc[d][2 * i + 1] * inv);
             }
-            if (p.a.lse && t4 == 0) p.a.lse[row * p.a.H + h] = kv8_lse(mx[i] - kKv8Lift, l);
+            if (p.a.lse && t4 == 0) p.a.lse[row * p.a.H + h] = kv8_lse(kv8_base(mx[i]), l);
         } else {
             const uint64_t row = ((static_cast<uint64_t>(seq) * p.a.max_new + i0 + token) * p.a.H + h) * p.splits + split;
             float* part = p.part + row * HD;
@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(kKpThreads) kv8_prefill_kernel(const Kv8Split 
                 part[8 * d + 2 * t4 + 1] = acc[d][2 * i + 1];
             }
             if (t4 == 0) {
-                p.part_ml[row * 2] = mx[i] - kKv8Lift;
+                p.part_ml[row * 2] = kv8_base(mx[i]);
                 p.part_ml[row * 2 + 1] = sum[i];
             }
         }

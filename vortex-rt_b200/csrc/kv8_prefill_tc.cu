@@ -26,7 +26,9 @@
 // fp32 and divided by that ratio again, one FMA for 32 keys.
 // The running maximum moves only when it grows by more than kTcSlack (base 2):
 // weights are then up to 2^(kTcLift + kTcSlack), within fp16, and O is seldom
-// rescaled (a rescale waits for the tensor cores: 2500 cycles).  What falls
+// rescaled (a rescale waits for the tensor cores: 2500 cycles).  Beyond kTcFar
+// the FMA, which does not round the score, would part from the maximum, which
+// is a rounded score, by whole numbers: there scores are rounded first.  What falls
 // under fp16's smallest step is 2^-28 of the largest weight times the largest
 // value, far below half a step of a 16-bit output.
 #include <cuda_runtime.h>
@@ -41,6 +43,7 @@
 namespace vrt {
 
 constexpr float kTcSlack = 12.0f, kTcLift = 3.0f;
+constexpr float kTcFar = 1048576.0f;  // scores (base 2) whose fp32 step is an eighth
 
 template <int HD>
 struct TcShape {
@@ -369,6 +372,7 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
         const int whole_c = min(stop, static_cast<int>(span.a) - static_cast<int>(span.b0) +
                                           static_cast<int>(max(static_cast<int64_t>(0), min(tile0 + 1, span.len)) / kKv8Page));
         float mx = -INFINITY, sum = 0.0f;
+        bool far = false;  // a row of the warp has its maximum beyond kTcFar
         const int mine = need[t];
         for (int j = 0; j < mine; ++j) {
             const int buf = 2 * t + (j & 1);
@@ -424,6 +428,7 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
             if (__any_sync(0xffffffffu, grown)) {
                 const float f = grown ? (mx == -INFINITY ? 0.0f : ex2(mx - top)) : 1.0f;
                 if (grown) mx = top;
+                far = __any_sync(0xffffffffu, mx > kTcFar || (mx < -kTcFar && mx != -INFINITY));
                 sum *= f;
                 if (j > 0) {
                     // P V of key tile j - 1 is done when S of j + 1, issued behind it, is
@@ -446,10 +451,11 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
                     tmem_wait_st();
                 }
             }
-            const float base = kTcLift - (mx == -INFINITY ? 0.0f : mx);
-            // kHidden: scores of -inf among them, which a tanh would make finite
-            auto weigh = [&](int c, const uint32_t(&v)[32], float a, float b, float inv, auto kHidden) {
+            const float seen = mx == -INFINITY ? 0.0f : mx, base = kTcLift - seen;
+            // kHidden: scores of -inf among them, which a tanh would make finite; kFar: scores beyond kTcFar
+            auto weigh = [&](int c, const uint32_t(&v)[32], float a, float b, float inv, auto kHidden, auto kFar) {
                 uint32_t w[16];
+                const float lifted = b + kTcLift;
                 b += base;
                 // CAP: cap * tanh(y) = cap - 2 cap / (e^2y + 1)
                 const float ca = a * (inv_cap * 2.0f * kLog2e), c1 = p.a.softcap * kLog2e + b, c2 = -2.0f * kLog2e * p.a.softcap;
@@ -467,7 +473,12 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
                             y = s1 == -INFINITY ? s1 : y;
                         }
                     } else {
-                        unpair(fma2(pair(x, y), a2, b2), x, y);
+                        if (decltype(kFar)::value) {
+                            x = __fsub_rn(__fmul_rn(x, a), seen) + lifted;
+                            y = __fsub_rn(__fmul_rn(y, a), seen) + lifted;
+                        } else {
+                            unpair(fma2(pair(x, y), a2, b2), x, y);
+                        }
                     }
                     if (CAP) {  // two special functions are spent on the tanh already
                         ex2_fma(x, y);
@@ -485,11 +496,14 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
                 tmem_st16(s_col + 16 * c, w);
             };
             if (CAP && !whole) {
-                weigh(0, va, a0, b0, i0v, std::true_type{});
-                weigh(1, vb, a1, b1, i1v, std::true_type{});
+                weigh(0, va, a0, b0, i0v, std::true_type{}, std::false_type{});
+                weigh(1, vb, a1, b1, i1v, std::true_type{}, std::false_type{});
+            } else if (!CAP && far) {
+                weigh(0, va, a0, b0, i0v, std::false_type{}, std::true_type{});
+                weigh(1, vb, a1, b1, i1v, std::false_type{}, std::true_type{});
             } else {
-                weigh(0, va, a0, b0, i0v, std::false_type{});
-                weigh(1, vb, a1, b1, i1v, std::false_type{});
+                weigh(0, va, a0, b0, i0v, std::false_type{}, std::false_type{});
+                weigh(1, vb, a1, b1, i1v, std::false_type{}, std::false_type{});
             }
             tmem_wait_st();
             tc_fence_before();
