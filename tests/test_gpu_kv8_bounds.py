@@ -1,5 +1,5 @@
 """Where 16-bit attention over the paged 8-bit KV cache can lose a result:
-scores far from 0.  Against plain implementations in 64 bits, as in
+scores far from 0, large score caps.  Against plain implementations in 64 bits, as in
 test_gpu_kv8.py, with tolerances that depend on what a row sees alone."""
 
 import math
@@ -53,6 +53,10 @@ def exact(c, i, q, pos, window=0, prefix=0, cap=0.0, tc=False):
     tol = HALF[c.dtype] * out.abs() + fi.tiny * fi.eps / 2 + amount * (2 * ds + sums + weight)[..., None]
     cut = torch.einsum("mt,thd->mhd", see.double(), vz.abs()) * w.amax(2)[..., None]
     tol = tol + (2.0 ** -28 if tc else 2.0 ** -39) * cut
+    # twice a weight's error is exp(2 ds) - 1 <= 4 ds only for ds <= 1/2; where scores are so large that theirs is
+    # beyond 1/4, any weights are right that are none below 0 and sum to 1: an output lies among the values seen
+    most = torch.where(see[:, :, None, None], vz.abs()[None], 0.0).amax(1) * (1 + 4 * HALF[c.dtype])
+    tol = torch.where((ds > 0.25)[..., None], out.abs() + most, tol)
     return out, lse, tol, ds + sums + lse.abs().nan_to_num(0, 0, 0) * U
 
 
@@ -95,3 +99,28 @@ def test_huge_scores(ctx, heads, dtype, far):
     # lse: the score, whose products' sum may be cut at each of hd additions
     top = torch.einsum("mhd,hd->mh", q[-1:].double(), c.values(0)[0][33].repeat_interleave(c.h // c.kv, 0)) * c.hd ** -0.5
     near(lse if row == m - 1 else c.decode(q[-1:])[1], top, (c.hd + 24) * U * top.abs(), "lse")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cap", [127.0, 129.0, 1e3, 1e4, 1e5, 1e8, 3e38])
+@pytest.mark.parametrize("heads", [(8, 2, 64), (8, 2, 128), (4, 1, 256)])
+def test_large_caps(ctx, heads, dtype, cap):
+    """A cap far above the scores leaves them as they are; scores near it and above it are bent."""
+    n, m = 300, 150
+    c = Cache(ctx, heads, dtype, [n])
+    g = torch.Generator("cuda").manual_seed(21)
+    c.append([(c.random(n, g), c.random(n, g))])
+    # ordinary scores, and (as far as the type holds the query) scores of the cap's size
+    for size in {2.0, min(2.0 * cap, 3e3 if dtype == "f16" else 1e30)}:
+        q = c.queries(m, g, size)
+        for few in (False, True):  # 64 dims: few rows take the warp form, more the tcgen05 form
+            rows = slice(m - 20, m) if few else slice(0, m)
+            out, lse = c.prefill(q[rows], [20 if few else m], cap=cap)
+            ro, rl, to, tl = exact(c, 0, q[rows], range(n - m, n)[rows], cap=cap, tc=uses_tc(c, 20 if few else m))
+            near(out, ro, to, f"prompt, {size}")
+            near(lse, rl, tl, f"lse of the prompt, {size}")
+        out, lse = c.decode(q[m - 1:], cap=cap)
+        ro, rl, to, tl = exact(c, 0, q[m - 1:], [n - 1], cap=cap)
+        near(out, ro, to, f"token, {size}")
+        near(lse, rl, tl, f"lse of the token, {size}")
+    assert status(ctx) == 0

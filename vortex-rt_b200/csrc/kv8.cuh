@@ -227,13 +227,20 @@ __device__ __forceinline__ uint32_t pack_half(__half a, __half b) {
     return static_cast<uint32_t>(__half_as_ushort(a)) | static_cast<uint32_t>(__half_as_ushort(b)) << 16;
 }
 
-// softcap * tanh(x / softcap), in base-2 units.  f32 rows take tanhf; for 16-bit
-// rows 1 - 2 / (1 + e^2y) is off by some 2^-22 of the cap, far below a weight's rounding.
-template <bool EXACT>
-__device__ __forceinline__ float capped(float x, float cap, float inv_cap) {
-    if (EXACT) return cap * tanhf(x * inv_cap) * kLog2e;
+// softcap * tanh(x / softcap), in base-2 units.  f32 rows take tanhf, off by a
+// few steps of the score.  16-bit rows take cap - 2 cap / (1 + e^2y), two special
+// functions, whose difference is off by some 2^-23 of the cap whatever the
+// score: up to a cap of 128 that is 2^-16 at most, far below a weight's rounding
+// (2^-11).  Larger caps take tanhf for all rows.
+constexpr float kKv8FastCap = 128.0f;
+__device__ __forceinline__ float capped_fast(float x, float cap, float inv_cap) {
     const float e = ex2(x * inv_cap * (2.0f * kLog2e));
     return cap * kLog2e * (1.0f - __fdividef(2.0f, e + 1.0f));
+}
+__device__ __forceinline__ float capped_exact(float x, float cap, float inv_cap) { return cap * tanhf(x * inv_cap) * kLog2e; }
+template <bool EXACT>
+__device__ __forceinline__ float capped(float x, float cap, float inv_cap) {
+    return EXACT || cap > kKv8FastCap ? capped_exact(x, cap, inv_cap) : capped_fast(x, cap, inv_cap);
 }
 
 // Splits of one (sequence, head) at most: the joining kernel's weights.

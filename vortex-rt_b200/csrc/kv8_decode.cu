@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(kKdThreads, KdShape<HD>::kCtas) kv8_decode_ker
     }
     __syncthreads();
     const int head0 = kPacked ? (2 * t4) % 4 : 2 * t4;  // heads of this lane's two columns
-    const bool plain_cap = p.a.softcap > 0.0f;
+    const bool plain_cap = p.a.softcap > 0.0f, fast_cap = TERMS == 1 && plain_cap && p.a.softcap <= kKv8FastCap;
     const float unit = plain_cap ? 1.0f : kLog2e, inv_cap = plain_cap ? 1.0f / p.a.softcap : 0.0f;
     const float sc[2] = {q_unit[head0] * (p.a.scale * unit), q_unit[head0 + 1] * (p.a.scale * unit)};
 
@@ -238,6 +238,18 @@ __global__ void __launch_bounds__(kKdThreads, KdShape<HD>::kCtas) kv8_decode_ker
                 for (int e = 0; e < 4; ++e) s[m][e] += __shfl_xor_sync(0xffffffffu, s[m][e], 2);
         }
         // ---- softmax: s[m][2 r + h] is block 2 m + r, this lane's head h
+        auto each = [&](auto f) {  // f(score, head)
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) s[b >> 1][2 * (b & 1) + h] = f(s[b >> 1][2 * (b & 1) + h], h);
+        };
+        each([&](float z, int h) { return z * (ks * sc[h]); });
+        if (fast_cap) {
+            each([&](float z, int) { return capped_fast(z, p.a.softcap, inv_cap); });
+        } else if (plain_cap) {
+            each([&](float z, int) { return capped_exact(z, p.a.softcap, inv_cap); });
+        }
         float top[2] = {mx[0], mx[1]};
         const bool full = there && (t0 + 32 <= span.prefix || (t0 >= span.lo && t0 + 32 <= span.len));
 #pragma unroll
@@ -247,8 +259,6 @@ __global__ void __launch_bounds__(kKdThreads, KdShape<HD>::kCtas) kv8_decode_ker
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 float& z = s[b >> 1][2 * (b & 1) + h];
-                z = z * (ks * sc[h]);
-                if (plain_cap) z = capped<TERMS == 2>(z, p.a.softcap, inv_cap);
                 if (!see) z = -INFINITY;
                 top[h] = fmaxf(top[h], z);
             }

@@ -244,7 +244,8 @@ __device__ __forceinline__ void tmem_arrived(uint32_t (&a)[32], uint32_t (&b)[32
     for (int c = 0; c < 32; ++c) asm volatile("" : "+r"(a[c]), "+r"(b[c]));
 }
 
-template <typename T, int HD, bool CAP>
+// CAP: 0 plain scores, 1 capped up to kKv8FastCap, 2 capped above it (tanhf)
+template <typename T, int HD, int CAP>
 __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kernel(const Kv8Split p) {
     using Shape = TcShape<HD>;
     constexpr int MT = Shape::MT, KT = Shape::KT, KB = Shape::KB, SUB = Shape::SUB, PG = Shape::PG, ST = Shape::kStages;
@@ -421,7 +422,8 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
                     for (int q = 0; q < 4; ++q) m4[q] = fmaxf(m4[q], fmaxf(__uint_as_float(v[i + q]), __uint_as_float(v[i + q + 4])));
                 }
                 const float z = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-                return z == -INFINITY ? z : CAP ? capped<false>(z * a, p.a.softcap, inv_cap) : z * a;
+                if (CAP == 0 || z == -INFINITY) return z == -INFINITY ? z : z * a;
+                return CAP == 1 ? capped_fast(z * a, p.a.softcap, inv_cap) : capped_exact(z * a, p.a.softcap, inv_cap);
             };
             const float top = fmaxf(highest(va, a0), highest(vb, a1));
             const bool grown = top > mx + kTcSlack;  // also from -inf
@@ -457,7 +459,7 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
                 uint32_t w[16];
                 const float lifted = b + kTcLift;
                 b += base;
-                // CAP: cap * tanh(y) = cap - 2 cap / (e^2y + 1)
+                // CAP 1: cap * tanh(y) = cap - 2 cap / (e^2y + 1)
                 const float ca = a * (inv_cap * 2.0f * kLog2e), c1 = p.a.softcap * kLog2e + b, c2 = -2.0f * kLog2e * p.a.softcap;
                 const uint64_t a2 = pair(a, a), b2 = pair(b, b);
                 uint64_t part[2] = {0, 0};
@@ -466,8 +468,14 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
                     float x = __uint_as_float(v[e]), y = __uint_as_float(v[e + 1]);
                     if (CAP) {
                         const float s0 = x, s1 = y;
-                        x = fmaf(rcp_approx(ex2(x * ca) + 1.0f), c2, c1);
-                        y = fmaf(rcp_approx(ex2(y * ca) + 1.0f), c2, c1);
+                        if (CAP == 1) {
+                            x = fmaf(rcp_approx(ex2(x * ca) + 1.0f), c2, c1);
+                            y = fmaf(rcp_approx(ex2(y * ca) + 1.0f), c2, c1);
+                        } else {
+                            // scores up to the cap, and beyond kTcFar: cut, as tanhf of a lower score may round higher
+                            x = fminf(__fsub_rn(capped_exact(x * a, p.a.softcap, inv_cap), seen) + lifted, kTcLift + kTcSlack);
+                            y = fminf(__fsub_rn(capped_exact(y * a, p.a.softcap, inv_cap), seen) + lifted, kTcLift + kTcSlack);
+                        }
                         if (decltype(kHidden)::value) {
                             x = s0 == -INFINITY ? s0 : x;
                             y = s1 == -INFINITY ? s1 : y;
@@ -480,7 +488,7 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
                             unpair(fma2(pair(x, y), a2, b2), x, y);
                         }
                     }
-                    if (CAP) {  // two special functions are spent on the tanh already
+                    if (CAP == 1) {  // two special functions are spent on the tanh already
                         ex2_fma(x, y);
                     } else {
                         x = ex2(x);
@@ -730,7 +738,7 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
 
 // -------------------------------------------------------------------- host
 
-template <typename T, int HD, bool CAP>
+template <typename T, int HD, int CAP>
 static cudaError_t tc_launch(const Kv8Split& p, cudaStream_t s) {
     using Shape = TcShape<HD>;
     static std::mutex mu;
@@ -756,12 +764,16 @@ static cudaError_t tc_launch(const Kv8Split& p, cudaStream_t s) {
 uint32_t kv8_prefill_tc_rows(uint32_t hd) { return hd == 256 ? 128u : 256u; }
 
 cudaError_t kv8_prefill_tc(const Kv8Split& p, uint32_t hd, cudaStream_t s) {
-    const bool cap = p.a.softcap > 0.0f;
-#define VRT_TC(HD)                                                              \
-    if (hd == HD) {                                                             \
-        if (p.a.dtype == VRT_F16) return cap ? tc_launch<__half, HD, true>(p, s) : tc_launch<__half, HD, false>(p, s); \
-        if (p.a.dtype == VRT_BF16)                                              \
-            return cap ? tc_launch<__nv_bfloat16, HD, true>(p, s) : tc_launch<__nv_bfloat16, HD, false>(p, s);         \
+    const int cap = p.a.softcap > kKv8FastCap ? 2 : p.a.softcap > 0.0f ? 1 : 0;
+#define VRT_TC(HD)                                                                                                  \
+    if (hd == HD) {                                                                                                 \
+        if (p.a.dtype == VRT_F16) {                                                                                 \
+            return cap == 2 ? tc_launch<__half, HD, 2>(p, s) : cap ? tc_launch<__half, HD, 1>(p, s) : tc_launch<__half, HD, 0>(p, s); \
+        }                                                                                                           \
+        if (p.a.dtype == VRT_BF16) {                                                                                \
+            return cap == 2 ? tc_launch<__nv_bfloat16, HD, 2>(p, s)                                                 \
+                            : cap ? tc_launch<__nv_bfloat16, HD, 1>(p, s) : tc_launch<__nv_bfloat16, HD, 0>(p, s);  \
+        }                                                                                                           \
     }
     VRT_TC(64) VRT_TC(128) VRT_TC(256)
 #undef VRT_TC
