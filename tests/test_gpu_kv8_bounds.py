@@ -1,5 +1,5 @@
 """Where 16-bit attention over the paged 8-bit KV cache can lose a result:
-scores far from 0, large score caps.  Against plain implementations in 64 bits, as in
+scores far from 0, large and tiny score caps.  Against plain implementations in 64 bits, as in
 test_gpu_kv8.py, with tolerances that depend on what a row sees alone."""
 
 import math
@@ -123,4 +123,31 @@ def test_large_caps(ctx, heads, dtype, cap):
         ro, rl, to, tl = exact(c, 0, q[m - 1:], [n - 1], cap=cap)
         near(out, ro, to, f"token, {size}")
         near(lse, rl, tl, f"lse of the token, {size}")
+    assert status(ctx) == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cap", [1e-20, 1e-38, 1e-42])
+@pytest.mark.parametrize("heads", [(8, 2, 64), (8, 2, 128), (4, 1, 256)])
+def test_tiny_caps(ctx, heads, dtype, cap):
+    """A cap whose reciprocal, or that times a score, is beyond fp32: all weights are the same, of scores of 0 too."""
+    n, m = 100, 70
+    c = Cache(ctx, heads, dtype, [n])
+    g = torch.Generator("cuda").manual_seed(23)
+    k, v = c.random(n, g), c.random(n, g)
+    k[7] = 0
+    k[64:96] = 0  # a page of zeros: its scale is 0
+    c.append([(k, v)])
+    q = c.queries(m, g, 300.0)
+    q[::3] = 0
+    ro, rl, to, tl = exact(c, 0, q, range(n - m, n), cap=cap, tc=True)
+    for few in (False, True):
+        rows = slice(m - 20, m) if few else slice(0, m)
+        out, lse = c.prefill(q[rows], [20 if few else m], cap=cap)
+        near(out, ro[rows], to[rows], "prompt")
+        near(lse, rl[rows], tl[rows], "lse of the prompt")
+    for row in (m - 1, m - 2):  # a query of zeros is among them
+        out, lse = c.decode(q[row:row + 1], cap=cap, lens=[n - m + row + 1])
+        near(out, ro[row:row + 1], to[row:row + 1], "token")
+        near(lse, rl[row:row + 1], tl[row:row + 1], "lse of the token")
     assert status(ctx) == 0

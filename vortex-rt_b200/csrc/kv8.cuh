@@ -233,6 +233,8 @@ __device__ __forceinline__ uint32_t pack_half(__half a, __half b) {
 // score: up to a cap of 128 that is 2^-16 at most, far below a weight's rounding
 // (2^-11).  Larger caps take tanhf for all rows.
 constexpr float kKv8FastCap = 128.0f;
+// 1 / cap, finite for the smallest caps too, and times 2 log2(e): a score of 0 stays 0
+__device__ __forceinline__ float kv8_inv_cap(float cap) { return fminf(1.0f / cap, 1.0e38f); }
 __device__ __forceinline__ float capped_fast(float x, float cap, float inv_cap) {
     const float e = ex2(x * inv_cap * (2.0f * kLog2e));
     return cap * kLog2e * (1.0f - __fdividef(2.0f, e + 1.0f));

@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(kKdThreads, KdShape<HD>::kCtas) kv8_decode_ker
     __syncthreads();
     const int head0 = kPacked ? (2 * t4) % 4 : 2 * t4;  // heads of this lane's two columns
     const bool plain_cap = p.a.softcap > 0.0f, fast_cap = TERMS == 1 && plain_cap && p.a.softcap <= kKv8FastCap;
-    const float unit = plain_cap ? 1.0f : kLog2e, inv_cap = plain_cap ? 1.0f / p.a.softcap : 0.0f;
+    const float unit = plain_cap ? 1.0f : kLog2e, inv_cap = plain_cap ? kv8_inv_cap(p.a.softcap) : 0.0f;
     const float sc[2] = {q_unit[head0] * (p.a.scale * unit), q_unit[head0 + 1] * (p.a.scale * unit)};
 
     float acc[KS][4];

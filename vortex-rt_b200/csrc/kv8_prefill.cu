@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(kKpThreads) kv8_prefill_kernel(const Kv8Split 
     }
     __syncthreads();
     const bool cap = p.a.softcap > 0.0f;
-    const float factor = cap ? p.a.scale : p.a.scale * kLog2e, inv_cap = cap ? 1.0f / p.a.softcap : 0.0f;
+    const float factor = cap ? p.a.scale : p.a.scale * kLog2e, inv_cap = cap ? kv8_inv_cap(p.a.softcap) : 0.0f;
     float sc[2];
     int64_t pos[2], lo[2];  // this lane's rows 16 warp + g8 (+ 8)
 #pragma unroll

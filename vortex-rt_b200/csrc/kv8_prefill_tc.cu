@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full);
         }
-        const float factor = CAP ? unit : unit * kLog2e, inv_cap = CAP ? 1.0f / p.a.softcap : 0.0f;
+        const float factor = CAP ? unit : unit * kLog2e, inv_cap = CAP ? kv8_inv_cap(p.a.softcap) : 0.0f;
         const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // this warp's 32 TMEM lanes
         const int64_t tile0 = pos0 + t * per, tile1 = pos0 + min((t + 1) * per, tokens) - 1;
         const int64_t lo1 = kv8_window_lo(tile1, p.a.window);
@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
                 const float lifted = b + kTcLift;
                 b += base;
                 // CAP 1: cap * tanh(y) = cap - 2 cap / (e^2y + 1)
-                const float ca = a * (inv_cap * 2.0f * kLog2e), c1 = p.a.softcap * kLog2e + b, c2 = -2.0f * kLog2e * p.a.softcap;
+                const float ca = fminf(a * (inv_cap * 2.0f * kLog2e), 3e38f), c1 = p.a.softcap * kLog2e + b, c2 = -2.0f * kLog2e * p.a.softcap;
                 const uint64_t a2 = pair(a, a), b2 = pair(b, b);
                 uint64_t part[2] = {0, 0};
 #pragma unroll
