@@ -1,6 +1,7 @@
 """Where 16-bit attention over the paged 8-bit KV cache can lose a result:
-scores far from 0, large and tiny score caps.  Against plain implementations in 64 bits, as in
-test_gpu_kv8.py, with tolerances that depend on what a row sees alone."""
+scores far from 0, large and tiny score caps, pages whose values are of very
+unlike size.  Against plain implementations in 64 bits, as in test_gpu_kv8.py,
+with tolerances that depend on what a row sees alone."""
 
 import math
 
@@ -151,3 +152,94 @@ def test_tiny_caps(ctx, heads, dtype, cap):
         near(out, ro[row:row + 1], to[row:row + 1], "token")
         near(lse, rl[row:row + 1], tl[row:row + 1], "lse of the token")
     assert status(ctx) == 0
+
+
+def unlike(c, n, g, places, times, base):
+    """Values of size `base`, and `times` that in the tokens of `places`."""
+    v = base * torch.randn((n, c.kv, c.hd), generator=g, device="cuda")
+    for a, b in places:
+        v[a:b] *= times
+    return v.to(TYPES[c.dtype])
+
+
+# (dtype, size of the ordinary values, how much larger the others are); fp16 holds 2^-24 to 2^16
+UNLIKE = [("f16", 2.0 ** -12, 2.0 ** 12), ("f16", 2.0 ** -14, 2.0 ** 24), ("f16", 2.0 ** -15, 2.0 ** 28),
+          ("bf16", 1.0, 2.0 ** 20), ("bf16", 2.0 ** -20, 2.0 ** 27), ("bf16", 1e-4, 2.0 ** 30), ("bf16", 1e-9, 2.0 ** 60),
+          ("bf16", 1e30, 2.0 ** -100), ("bf16", 1e-36, 1.0), ("f32", 1e-4, 2.0 ** 30)]
+
+
+@pytest.mark.parametrize("dtype,base,times", UNLIKE)
+@pytest.mark.parametrize("heads", [(8, 2, 64), (8, 2, 128), (3, 1, 128), (4, 1, 256)])
+@pytest.mark.parametrize("places", [[(96, 128)], [(0, 32)], [(70, 71), (200, 201)], [(290, 300)]])
+def test_values_of_unlike_size(ctx, heads, dtype, base, times, places):
+    """Values far larger or smaller than a row's own, in pages that it does not see (later ones, or behind its window),
+    in its own page, and in sight, where they decide."""
+    n = 300
+    c = Cache(ctx, heads, dtype, [n, 40])
+    g = torch.Generator("cuda").manual_seed(24)
+    c.append([(c.random(n, g), unlike(c, n, g, places, times, base)), (c.random(40, g), c.random(40, g))])
+    for window, prefix, cap in ((0, 0, 0.0), (40, 0, 0.0), (33, 5, 20.0), (0, 100, 500.0)):
+        q = c.queries(n + 40, g)
+        pre = [prefix, min(40, prefix)] if prefix else None
+        out, lse = c.prefill(q, [n, 40], window, pre, cap)
+        tc = uses_tc(c, n)
+        for i, (m, r) in enumerate(((n, 0), (40, n))):
+            ro, rl, to, tl = exact(c, i, q[r:r + m], range(m), window, pre[i] if pre else 0, cap, tc)
+            near(out[r:r + m], ro, to, f"window {window}, prefix {prefix}, cap {cap}")
+            near(lse[r:r + m], rl, tl, f"lse, window {window}, prefix {prefix}, cap {cap}")
+        out, lse = c.decode(q[[n - 1, n + 39]], window, pre, cap)
+        for i, m in enumerate((n, 40)):
+            ro, rl, to, tl = exact(c, i, q[[(n - 1, n + 39)[i]]], [m - 1], window, pre[i] if pre else 0, cap)
+            near(out[i:i + 1], ro, to, "token")
+            near(lse[i:i + 1], rl, tl, "lse of the token")
+    assert status(ctx) == 0
+
+
+@pytest.mark.parametrize("dtype,base,times", [("f16", 2.0 ** -14, 2.0 ** 24), ("bf16", 1.0, 2.0 ** 40)])
+@pytest.mark.parametrize("heads", [(8, 2, 64), (8, 2, 128), (10, 2, 256)])
+def test_values_of_unlike_size_split(ctx, heads, dtype, base, times):
+    """The same behind a long history that is split: parts whose scales are alike beside parts whose are not."""
+    n, m = 3001, 140
+    c = Cache(ctx, heads, dtype, [n])
+    g = torch.Generator("cuda").manual_seed(25)
+    c.append([(c.random(n, g), unlike(c, n, g, [(1000, 1032), (2900, 2901)], times, base))])
+    q = c.queries(m, g)
+    for window, prefix in ((0, 0), (1900, 0), (90, 0), (64, 999)):
+        out, lse = c.prefill(q, [m], window, [prefix] if prefix else None)
+        ro, rl, to, tl = exact(c, 0, q, range(n - m, n), window, prefix, tc=True)
+        near(out, ro, to, f"window {window}, prefix {prefix}")
+        near(lse, rl, tl, f"lse, window {window}, prefix {prefix}")
+    again, _ = c.prefill(q, [m], 64, [999])
+    assert torch.equal(out, again)
+
+
+@pytest.mark.parametrize("heads,dtype", [((8, 2, 128), "bf16"), ((4, 1, 256), "f16"), ((8, 1, 64), "bf16")])
+@pytest.mark.parametrize("times", [1.0, 2.0 ** 20, 2.0 ** 35])
+def test_values_of_unlike_size_missing_page(ctx, heads, dtype, times):
+    """A page that is not in the pool beside pages of unlike value size: rows in front of it are as before."""
+    n = 300
+    c = Cache(ctx, heads, dtype, [n])
+    g = torch.Generator("cuda").manual_seed(26)
+    c.append([(c.random(n, g), unlike(c, n, g, [(128, 160)], times, 2.0 ** -22 if dtype == "f16" else 1.0))])
+    q = c.queries(n, g)
+    good, _ = c.prefill(q, [n])
+    c.table[0, 3] = c.pages
+    out, lse = c.prefill(q, [n])
+    assert status(ctx) == 32
+    assert torch.equal(out[:96], good[:96]) and torch.isfinite(out).all() and torch.isfinite(lse).all()
+
+
+def test_foreign_value_scales(ctx):
+    """Scales that no append makes, in arrays that a program filled itself: negative, and near both ends of fp32."""
+    c = Cache(ctx, (8, 2, 128), "bf16", [200])
+    g = torch.Generator("cuda").manual_seed(27)
+    c.append([(c.random(200, g), c.random(200, g))])
+    q = c.queries(200, g)
+    good, lse = c.prefill(q, [200])
+    keep = c.vs.clone()
+    for f in (-1.0, 2.0 ** -100, 2.0 ** 119):
+        c.vs.copy_(keep * f)
+        out, l2 = c.prefill(q, [200])
+        # exact products by a power of two, until fp32's subnormal numbers: 2^-100 is not near them
+        near(out.double() / f, good.double(), good.double().abs() * 2.0 ** -7 + 2.0 ** -9 * good.double().abs().max(), f"{f}")
+        near(l2, lse.double(), torch.full_like(lse, 1e-4).double(), f"lse, {f}")

@@ -20,17 +20,22 @@
 //
 // Scales: a page's key scale and the row's factor are one FMA in front of the
 // exponential.  A page's value scale cannot be taken out of O, which sums over
-// pages: the weight is multiplied by v_scale / (largest v_scale that the CTA
-// sees) in the same FMA, as an addend to the exponent, so that the codes stay
-// exact and a weight is rounded once.  The sum of weights is kept by page in
-// fp32 and divided by that ratio again, one FMA for 32 keys.
+// pages: it is 2^e f with f in [1/2, 1).  The codes are stored times 2^e, counted
+// from the largest value scale of the CTA's pages, which fp16 holds exactly down
+// to 2^-28 of that (8 bits of code on its smallest step, 2^-24); the weight is
+// multiplied by f in the FMA in front of its exponential, as an addend, and is
+// rounded once.  So how large the values are that a row does not see, or hardly
+// weighs, costs its own no bit.  The sum of weights is kept by page in fp32 and
+// divided by f again, one FMA for 32 keys.  Pages whose value scales lie further
+// apart than 2^28, or close to fp32's ends, take the form that follows below:
+// scores and products of a row on its thread's fp32 pipes, O still in TMEM.
 // The running maximum moves only when it grows by more than kTcSlack (base 2):
 // weights are then up to 2^(kTcLift + kTcSlack), within fp16, and O is seldom
 // rescaled (a rescale waits for the tensor cores: 2500 cycles).  Beyond kTcFar
 // the FMA, which does not round the score, would part from the maximum, which
 // is a rounded score, by whole numbers: there scores are rounded first.  What falls
-// under fp16's smallest step is 2^-28 of the largest weight times the largest
-// value, far below half a step of a 16-bit output.
+// under fp16's smallest step is 2^-28 of a row's largest weight, times values that
+// the row sees, each its own: far below half a step of a 16-bit output.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -42,8 +47,16 @@
 
 namespace vrt {
 
-constexpr float kTcSlack = 12.0f, kTcLift = 3.0f;
+constexpr float kTcSlack = 11.0f, kTcLift = 4.0f;
 constexpr float kTcFar = 1048576.0f;  // scores (base 2) whose fp32 step is an eighth
+
+// Value scales by the exponent field of their fp32: the largest of a CTA's
+// pages within [kTcScaleLow, kTcScaleHigh], all others but zeros at most
+// kTcScaleSpan below.
+constexpr int kTcScaleLow = 40, kTcScaleHigh = 250, kTcScaleSpan = 28;
+constexpr int kTcCodeUp = 4;  // codes of the largest are stored times 2^4: 1152 * 2^4, their offset, is within fp16
+__device__ __forceinline__ int scale_exponent(float s) { return static_cast<int>(__float_as_uint(s) >> 23 & 255u); }
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
 
 template <int HD>
 struct TcShape {
@@ -69,8 +82,8 @@ struct TcShape {
 
 struct TcMeta {  // what the softmax knows of a page
     float k_scale;
-    float v_log;  // log2(v_scale / reference), 0 for a page of zeros
-    float v_inv;  // 2^-v_log
+    float v_log;  // log2 of f, the value scale's fraction in [1/2, 1); 0 for a page of zeros
+    float v_inv;  // 1 / f
     int there;
 };
 
@@ -217,6 +230,29 @@ __device__ __forceinline__ void store_codes(uint8_t* a, uint8_t* b, uint4 u) {
     *reinterpret_cast<uint4*>(b) = make_uint4(codes_lo(w[2]), codes_hi(w[2]), codes_lo(w[3]), codes_hi(w[3]));
 }
 
+// The same times `mul`, a power of two in both halves; off is -1152 times it (codes_lo, in one FMA).
+__device__ __forceinline__ uint32_t scaled_codes(uint32_t w, uint32_t bytes, __half2 mul, __half2 off) {
+    const uint32_t b = __byte_perm(w, 0x64646464u, bytes);
+    const __half2 h = __hfma2(*reinterpret_cast<const __half2*>(&b), mul, off);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void store_codes(uint8_t* a, uint8_t* b, uint4 u, __half2 mul, __half2 off) {
+    const uint32_t w[4] = {u.x ^ 0x80808080u, u.y ^ 0x80808080u, u.z ^ 0x80808080u, u.w ^ 0x80808080u};
+    uint32_t h[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        h[2 * i] = scaled_codes(w[i], 0x4140u, mul, off);
+        h[2 * i + 1] = scaled_codes(w[i], 0x4342u, mul, off);
+    }
+    *reinterpret_cast<uint4*>(a) = make_uint4(h[0], h[1], h[2], h[3]);
+    *reinterpret_cast<uint4*>(b) = make_uint4(h[4], h[5], h[6], h[7]);
+}
+
+// The four codes of a word whose bytes were offset by 128, as fp32: a byte under the exponent of 2^23.
+__device__ __forceinline__ float code_f32(uint32_t w, int i) {
+    return __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7550u + i)) - 8388736.0f;
+}
+
 template <int N>
 __device__ __forceinline__ void more_registers() {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -267,8 +303,11 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
     uint64_t* o_last = p_full + 4;   // [tile][2] the last P V but one and the last are added
     uint64_t* drained = o_last + 4;  // [tile] after a wait gave up: the MMAs in flight are done
     TcMeta* meta = reinterpret_cast<TcMeta*>(drained + 2);           // [4][PG]
-    float* reference = reinterpret_cast<float*>(meta + 4 * PG);     // [4 warps], then the value scale that O counts in
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(reference + 5);
+    float* unit_v = reinterpret_cast<float*>(meta + 4 * PG);  // what O counts in
+    int* v_top = reinterpret_cast<int*>(unit_v + 1);          // [4 warps] the value scales' largest exponent field
+    int* v_low = v_top + 4;                                   // [4 warps] and smallest, 0 if a scale is out of range
+    volatile int* wide = reinterpret_cast<volatile int*>(v_low + 4);  // scales too far apart for fp16 codes
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_low + 5);
     volatile int* missing = reinterpret_cast<volatile int*>(tmem_slot + 1);  // a page was not in the pool
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -313,6 +352,7 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
         }
         for (int t = 0; t < 2; ++t) mbar_init(drained + t, 1);
         *missing = 0;
+        *wide = 0;
         fence_mbar_init();
     }
     if (warp == 4 * MT + 8) tmem_alloc(tmem_slot, 512);
@@ -375,7 +415,84 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
         float mx = -INFINITY, sum = 0.0f;
         bool far = false;  // a row of the warp has its maximum beyond kTcFar
         const int mine = need[t];
-        for (int j = 0; j < mine; ++j) {
+        // the keys of a page at t0 that the row sees, a bit each
+        auto visible = [&](int t0) {
+            auto below = [](int x) { return x >= 32 ? 0xffffffffu : x <= 0 ? 0u : (1u << x) - 1u; };
+            return (below(end - t0) & ~below(lo - t0)) | below(prefix - t0);
+        };
+        bool slow = false;
+        if (J > 0) {
+            named_bar_sync(2, Shape::kThreads);  // the value scales have been looked through
+            slow = *wide;
+        }
+        if (slow) {
+            const uint32_t at_o = tmem + lanes + Shape::kOCol + t * HD;
+            const int pages = min(2 * mine, static_cast<int>(j1 - j0));
+#pragma unroll 1
+            for (int i = 0; i < pages; ++i) {
+                const uint32_t page = span.page(j0 + i);
+                const int id = kv8_page(p.a.c, seq, page, p.a.status);
+                const uint64_t head = static_cast<uint64_t>(max(id, 0)) * p.a.c.kv + g;
+                const uint32_t see = id < 0 ? 0u : visible(static_cast<int>(page * kKv8Page));
+                const float kf = p.a.c.k_scale[head] * factor, vf = see ? p.a.c.v_scale[head] : 0.0f;
+                const uint8_t* kp = reinterpret_cast<const uint8_t*>(p.a.c.k + head * (kKv8Page * HD));
+                const uint8_t* vp = reinterpret_cast<const uint8_t*>(p.a.c.v + head * (kKv8Page * HD));
+                float w[kKv8Page];  // scores, then weights
+#pragma unroll
+                for (int k = 0; k < 32; ++k) w[k] = 0.0f;
+#pragma unroll 1
+                for (int d = 0; d < HD; d += 4) {
+                    const uint2 q4 = *reinterpret_cast<const uint2*>(sq + t * Shape::kQTile + d / 64 * (128 * 128) + sw128_offset(row, d % 64));
+                    const float2 q01 = __half22float2(*reinterpret_cast<const __half2*>(&q4.x));
+                    const float2 q23 = __half22float2(*reinterpret_cast<const __half2*>(&q4.y));
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) {
+                        const uint32_t c = __ldg(reinterpret_cast<const uint32_t*>(kp + k * HD + d)) ^ 0x80808080u;
+                        w[k] = fmaf(q01.x, code_f32(c, 0), w[k]);
+                        w[k] = fmaf(q01.y, code_f32(c, 1), w[k]);
+                        w[k] = fmaf(q23.x, code_f32(c, 2), w[k]);
+                        w[k] = fmaf(q23.y, code_f32(c, 3), w[k]);
+                    }
+                }
+                float top = mx;
+#pragma unroll
+                for (int k = 0; k < 32; ++k) {
+                    float z = w[k] * kf;
+                    if (CAP == 1) z = capped_fast(z, p.a.softcap, inv_cap);
+                    if (CAP == 2) z = capped_exact(z, p.a.softcap, inv_cap);
+                    w[k] = see >> k & 1 ? z : -INFINITY;
+                    top = fmaxf(top, w[k]);
+                }
+                const float f = mx == -INFINITY ? 0.0f : ex2(mx - top), from = top == -INFINITY ? 0.0f : top;
+                mx = top;
+                sum *= f;
+#pragma unroll
+                for (int k = 0; k < 32; ++k) {
+                    w[k] = ex2((w[k] - from) + kTcLift);
+                    sum += w[k];
+                }
+#pragma unroll 1
+                for (int d = 0; d < HD; d += 16) {
+                    uint32_t o[16] = {};
+                    if (i > 0) tmem_ld16(at_o + d, o);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const uint8_t* from_v = vp + (d + e) * static_cast<int>(kKv8Page);
+                        float x = 0.0f;
+#pragma unroll
+                        for (int k = 0; k < 32; k += 4) {
+                            const uint32_t c = __ldg(reinterpret_cast<const uint32_t*>(from_v + k)) ^ 0x80808080u;
+#pragma unroll
+                            for (int b = 0; b < 4; ++b) x = fmaf(w[k + b], code_f32(c, b), x);
+                        }
+                        o[e] = __float_as_uint(fmaf(x, vf, __uint_as_float(o[e]) * f));
+                    }
+                    tmem_st16(at_o + d, o);
+                    tmem_wait_st();
+                }
+            }
+        }
+        for (int j = 0; j < mine && !slow; ++j) {
             const int buf = 2 * t + (j & 1);
             const uint32_t s_col = tmem + lanes + buf * KT;
             ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded(s_full + buf, (j >> 1) & 1));
@@ -397,8 +514,7 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
                 // scale of a page that the row does not see is left out.
                 auto mask = [&](int c, uint32_t(&v)[32], float& a, float& b, float& inv) {
                     const int t0 = static_cast<int>(span.page(j0 + 2 * j + c) * kKv8Page);
-                    auto below = [](int x) { return x >= 32 ? 0xffffffffu : x <= 0 ? 0u : (1u << x) - 1u; };
-                    const uint32_t see = mt[c].there ? ((below(end - t0) & ~below(lo - t0)) | below(prefix - t0)) : 0u;
+                    const uint32_t see = mt[c].there ? visible(t0) : 0u;
                     const bool bad = !(a < INFINITY) || !(b <= 0.0f);
                     a = bad ? 1.0f : fmaxf(a, 1e-37f);
                     b = bad ? 0.0f : b;
@@ -519,12 +635,12 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
             if (lane == 0) mbar_arrive(p_full + buf);
         }
         // ---- output
-        if (mine > 0) {
+        if (mine > 0 && !slow) {
             ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded(o_last + 2 * t + 1, 0));
             tc_fence_after();
         }
         if (mx == -INFINITY && sum < INFINITY) sum = 0.0f;  // nothing seen: what ex2_fma makes of -inf
-        const float ref = mine > 0 ? reference[4] : 0.0f;
+        const float ref = mine > 0 ? (slow ? 1.0f : *unit_v) : 0.0f;
         const float mul = used == 1 ? (sum == 0.0f ? 0.0f : ref / sum) : ref;
         T* out = static_cast<T*>(p.a.out) + at * p.a.out_stride + static_cast<uint64_t>(h) * HD;
         const uint64_t prow = ((static_cast<uint64_t>(seq) * p.a.max_new + i0 + token) * p.a.H + h) * p.splits + split;
@@ -564,7 +680,6 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
         const int c0 = tid - 128 * (keys ? MT : MT + 1);
         constexpr int C = PG * HD * 2 / 128;  // 16-byte pieces of a block that a thread brings
         constexpr int kPieces = HD * 2 / 128; // of them in a page
-        float ref = 1.0f;
         // Piece i of a thread is 128 pieces behind piece i - 1: a whole number of the periods below, so its page, its
         // offset in the page and in the operand tile are constants away.  Pieces are dealt so that a quarter warp's
         // stores meet all banks: 64 dims of two keys; 4 dims of values from both halves of a swizzle period.
@@ -579,7 +694,9 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
         uint4 r[C];
         // pool index of each page of the block at hand and of the next: looked up a block ahead of the codes
         int ids[PG], ids_next[PG] = {};
-        float ks = 0.0f, vs = 0.0f;  // scales of page c0 (key threads c0 < PG)
+        const int mine_c = keys ? c0 : lane;  // the page of a block whose scales this thread knows, if below PG
+        float ks = 0.0f, vs = 0.0f;
+        int v_exp = 0;  // the CTA's largest value scale, its exponent field
         for (int j = -2; j < blocks_k; ++j) {  // store block j, ask for block j + 1, look block j + 2 up
             if (j >= 0) {
                 const int s = j % ST;
@@ -596,8 +713,9 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
                         if (e.there) {
                             e.k_scale = ks;
                             if (vs != 0.0f) {
-                                e.v_log = vs < INFINITY ? fmaxf(log2f(vs / ref), -60.0f) : NAN;
-                                e.v_inv = exp2f(-e.v_log);
+                                const float f = __uint_as_float((__float_as_uint(vs) & 0x7fffffu) | 0x3f000000u);
+                                e.v_log = vs < INFINITY ? log2f(f) : NAN;
+                                e.v_inv = vs < INFINITY ? 1.0f / f : NAN;
                             }
                         }
                         meta[(j & 3) * PG + c0] = e;
@@ -608,12 +726,19 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
                         store_codes(at + to + i * step, at + (to ^ 16u) + i * step, r[i]);
                     }
                 } else {
+                    // the power of two that the codes of page `lane` are stored times; 0 for a page of zeros or NaN
+                    const float up = vs > 0.0f && vs < INFINITY ? power_of_two(scale_exponent(vs) - v_exp + kTcCodeUp) : 0.0f;
+                    const __half2 up2 = __float2half2_rn(up);
+                    const uint32_t mul_l = *reinterpret_cast<const uint32_t*>(&up2);
+                    uint32_t mul = 0;
 #pragma unroll
                     for (int i = 0; i < C; ++i) {
+                        if (i % kPieces == 0) mul = __shfl_sync(0xffffffffu, mul_l, i / kPieces);
+                        const __half2 m2 = *reinterpret_cast<const __half2*>(&mul), off = __hmul2(m2, __float2half2_rn(-1152.0f));
                         // 64 dims of 128 pieces; a page's keys are half a swizzled row, two pages a row
                         const uint32_t v_to = to ^ (i / kPieces % 2 * 64u);
-                        const uint32_t off = i / kPieces / 2 * (HD * 128) + i % kPieces * (64 * 128);
-                        store_codes(at + v_to + off, at + (v_to ^ 16u) + off, r[i]);
+                        const uint32_t place = i / kPieces / 2 * (HD * 128) + i % kPieces * (64 * 128);
+                        store_codes(at + v_to + place, at + (v_to ^ 16u) + place, r[i], m2, off);
                     }
                 }
                 fence_proxy_async_smem();
@@ -641,29 +766,41 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
                     if (ids[c] >= 0) r[c * kPieces + i] = __ldg(reinterpret_cast<const uint4*>(from + i * 2048));
                 }
             }
-            if (keys && c0 < PG) {
+            if (mine_c < PG) {
                 int id = ids[0];
 #pragma unroll
-                for (int x = 1; x < PG; ++x) id = x == c0 ? ids[x] : id;
+                for (int x = 1; x < PG; ++x) id = x == mine_c ? ids[x] : id;
                 const uint64_t head = static_cast<uint64_t>(max(id, 0)) * p.a.c.kv + g;
                 ks = __ldg(p.a.c.k_scale + head);
-                vs = __ldg(p.a.c.v_scale + head);
+                vs = id < 0 ? 0.0f : __ldg(p.a.c.v_scale + head);  // a page that is not there is zeros
             }
-            if (keys && j == -1) {
-                // the largest value scale among the CTA's pages, while the first block's codes travel
-                float m = 0.0f;
-                for (uint32_t i = j0 + c0; i < j1; i += 128) {
-                    const int id = kv8_page(p.a.c, seq, span.page(i), p.a.status);
-                    const float v = id < 0 ? 0.0f : p.a.c.v_scale[static_cast<uint64_t>(id) * p.a.c.kv + g];
-                    if (v < INFINITY) m = fmaxf(m, v);
+            if (j == -1) {
+                if (keys) {
+                    // the value scales of the CTA's pages, while the first block's codes travel
+                    int top = 0, low = 255;
+                    for (uint32_t i = j0 + c0; i < j1; i += 128) {
+                        const int id = kv8_page(p.a.c, seq, span.page(i), p.a.status);
+                        const float v = id < 0 ? 0.0f : p.a.c.v_scale[static_cast<uint64_t>(id) * p.a.c.kv + g];
+                        if (v == 0.0f || !(v < INFINITY)) continue;
+                        top = max(top, scale_exponent(v));
+                        low = min(low, v > 0.0f ? scale_exponent(v) : 0);
+                    }
+                    top = __reduce_max_sync(0xffffffffu, top);
+                    low = __reduce_min_sync(0xffffffffu, low);
+                    if (lane == 0) v_top[warp - 4 * MT] = top, v_low[warp - 4 * MT] = low;
+                    named_bar_sync(1, 128);
+                    if (c0 == 0) {
+                        top = max(max(v_top[0], v_top[1]), max(v_top[2], v_top[3]));
+                        low = min(min(v_low[0], v_low[1]), min(v_low[2], v_low[3]));
+                        const bool some = low < 255;  // a scale that is not 0
+                        *wide = some && (top < kTcScaleLow || top > kTcScaleHigh || low < top - kTcScaleSpan);
+                        // codes times 2^kTcCodeUp, weights times f = scale / 2^(exponent + 1)
+                        *unit_v = some ? power_of_two(min(max(top, kTcScaleLow), kTcScaleHigh) - 126 - kTcCodeUp) : 1.0f;
+                    }
                 }
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                if (lane == 0) reference[warp - 4 * MT] = m;
-                named_bar_sync(1, 128);
-                m = fmaxf(fmaxf(reference[0], reference[1]), fmaxf(reference[2], reference[3]));
-                if (m > 0.0f) ref = m;
-                if (c0 == 0) reference[4] = ref;
+                named_bar_sync(2, Shape::kThreads);
+                if (*wide) break;
+                v_exp = max(max(v_top[0], v_top[1]), max(v_top[2], v_top[3]));
             }
         }
     } else {
@@ -671,8 +808,10 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
         fewer_registers<Shape::kRegsMma>();
         const int t = warp - (4 * MT + 8);
         if (t < MT) {
+            if (J > 0) named_bar_sync(2, Shape::kThreads);
             auto wait = [&](uint64_t* bar, int phase) { ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded(bar, phase & 1)); };
-            const int mine = t ? need[1] : need[0];
+            const bool none = J == 0 || *wide;  // no key tile, or none for the tensor cores
+            const int mine = none ? 0 : t ? need[1] : need[0];
             int k_seen = -1, v_seen = -1;  // blocks waited for
             const uint64_t qa = sw128_desc(smem_addr(sq + t * Shape::kQTile));
             if (mine > 0) wait(q_full, 0);
@@ -716,7 +855,7 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
                 }
             }
             // blocks that only the other row tile reads: given back as they come, so that each counts in its own phase
-            for (int blk = (mine + SUB - 1) / SUB; blk < blocks_k && ok; ++blk) {
+            for (int blk = (mine + SUB - 1) / SUB; blk < blocks_k && ok && !none; ++blk) {
                 wait(k_full + blk % ST, blk / ST);
                 if (lane == 0) mbar_arrive(k_empty + blk % ST);
                 wait(v_full + blk % ST, blk / ST);
@@ -726,6 +865,8 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
                 warp_commit(drained + t);
                 mbar_wait_bounded(drained + t, 0);
             }
+        } else if (J > 0) {
+            named_bar_sync(2, Shape::kThreads);
         }
     }
     if (!ok) atomicOr(p.a.status, kStatusWaitTimeout);
