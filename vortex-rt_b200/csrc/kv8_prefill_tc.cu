@@ -20,7 +20,7 @@
 //
 // Scales: a page's key scale and the row's factor are one FMA in front of the
 // exponential.  A page's value scale cannot be taken out of O, which sums over
-// pages: it is 2^e f with f in [1/2, 1).  The codes are stored times 2^e, counted
+// pages: it is 2^e f with f in [1/sqrt 2, sqrt 2).  The codes are stored times 2^e, counted
 // from the largest value scale of the CTA's pages, which fp16 holds exactly down
 // to 2^-28 of that (8 bits of code on its smallest step, 2^-24); the weight is
 // multiplied by f in the FMA in front of its exponential, as an addend, and is
@@ -30,7 +30,7 @@
 // apart than 2^28, or close to fp32's ends, take the form that follows below:
 // scores and products of a row on its thread's fp32 pipes, O still in TMEM.
 // The running maximum moves only when it grows by more than kTcSlack (base 2):
-// weights are then up to 2^(kTcLift + kTcSlack), within fp16, and O is seldom
+// weights are then up to 2^(kTcLift + kTcSlack), with f within fp16, and O is seldom
 // rescaled (a rescale waits for the tensor cores: 2500 cycles).  Beyond kTcFar
 // the FMA, which does not round the score, would part from the maximum, which
 // is a rounded score, by whole numbers: there scores are rounded first.  What falls
@@ -47,15 +47,18 @@
 
 namespace vrt {
 
-constexpr float kTcSlack = 11.0f, kTcLift = 4.0f;
+constexpr float kTcSlack = 11.5f, kTcLift = 3.5f;
 constexpr float kTcFar = 1048576.0f;  // scores (base 2) whose fp32 step is an eighth
 
 // Value scales by the exponent field of their fp32: the largest of a CTA's
 // pages within [kTcScaleLow, kTcScaleHigh], all others but zeros at most
 // kTcScaleSpan below.
 constexpr int kTcScaleLow = 40, kTcScaleHigh = 250, kTcScaleSpan = 28;
-constexpr int kTcCodeUp = 4;  // codes of the largest are stored times 2^4: 1152 * 2^4, their offset, is within fp16
+constexpr int kTcCodeUp = 4;  // codes of the largest are stored times 2^4 or 2^5: 1152 * 2^5, their offset, is within fp16
 __device__ __forceinline__ int scale_exponent(float s) { return static_cast<int>(__float_as_uint(s) >> 23 & 255u); }
+// The exponent field of the power of two that a scale is within [1/sqrt 2, sqrt 2) of, and how many times that it is.
+__device__ __forceinline__ int scale_power(float s) { return static_cast<int>(__float_as_uint(s) + 0x4afb0du >> 23); }
+__device__ __forceinline__ float scale_rest(float s) { return __uint_as_float(__float_as_uint(s) - (static_cast<uint32_t>(scale_power(s) - 127) << 23)); }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
 
 template <int HD>
@@ -82,7 +85,7 @@ struct TcShape {
 
 struct TcMeta {  // what the softmax knows of a page
     float k_scale;
-    float v_log;  // log2 of f, the value scale's fraction in [1/2, 1); 0 for a page of zeros
+    float v_log;  // log2 of f, what the value scale is of its power of two; 0 for a page of zeros
     float v_inv;  // 1 / f
     int there;
 };
@@ -425,7 +428,7 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
             named_bar_sync(2, Shape::kThreads);  // the value scales have been looked through
             slow = *wide;
         }
-        if (slow) {
+        if (__builtin_expect(slow, 0)) {
             const uint32_t at_o = tmem + lanes + Shape::kOCol + t * HD;
             const int pages = min(2 * mine, static_cast<int>(j1 - j0));
 #pragma unroll 1
@@ -515,7 +518,7 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
                 auto mask = [&](int c, uint32_t(&v)[32], float& a, float& b, float& inv) {
                     const int t0 = static_cast<int>(span.page(j0 + 2 * j + c) * kKv8Page);
                     const uint32_t see = mt[c].there ? visible(t0) : 0u;
-                    const bool bad = !(a < INFINITY) || !(b <= 0.0f);
+                    const bool bad = !(a < INFINITY) || !(b < INFINITY);
                     a = bad ? 1.0f : fmaxf(a, 1e-37f);
                     b = bad ? 0.0f : b;
                     inv = bad ? (see ? NAN : 1.0f) : inv;
@@ -589,8 +592,8 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
                             y = fmaf(rcp_approx(ex2(y * ca) + 1.0f), c2, c1);
                         } else {
                             // scores up to the cap, and beyond kTcFar: cut, as tanhf of a lower score may round higher
-                            x = fminf(__fsub_rn(capped_exact(x * a, p.a.softcap, inv_cap), seen) + lifted, kTcLift + kTcSlack);
-                            y = fminf(__fsub_rn(capped_exact(y * a, p.a.softcap, inv_cap), seen) + lifted, kTcLift + kTcSlack);
+                            x = fminf(__fsub_rn(capped_exact(x * a, p.a.softcap, inv_cap), seen), kTcSlack) + lifted;
+                            y = fminf(__fsub_rn(capped_exact(y * a, p.a.softcap, inv_cap), seen), kTcSlack) + lifted;
                         }
                         if (decltype(kHidden)::value) {
                             x = s0 == -INFINITY ? s0 : x;
@@ -622,7 +625,7 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
             if (CAP && !whole) {
                 weigh(0, va, a0, b0, i0v, std::true_type{}, std::false_type{});
                 weigh(1, vb, a1, b1, i1v, std::true_type{}, std::false_type{});
-            } else if (!CAP && far) {
+            } else if (!CAP && __builtin_expect(far, 0)) {
                 weigh(0, va, a0, b0, i0v, std::false_type{}, std::true_type{});
                 weigh(1, vb, a1, b1, i1v, std::false_type{}, std::true_type{});
             } else {
@@ -713,7 +716,7 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
                         if (e.there) {
                             e.k_scale = ks;
                             if (vs != 0.0f) {
-                                const float f = __uint_as_float((__float_as_uint(vs) & 0x7fffffu) | 0x3f000000u);
+                                const float f = scale_rest(vs);
                                 e.v_log = vs < INFINITY ? log2f(f) : NAN;
                                 e.v_inv = vs < INFINITY ? 1.0f / f : NAN;
                             }
@@ -727,7 +730,7 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
                     }
                 } else {
                     // the power of two that the codes of page `lane` are stored times; 0 for a page of zeros or NaN
-                    const float up = vs > 0.0f && vs < INFINITY ? power_of_two(scale_exponent(vs) - v_exp + kTcCodeUp) : 0.0f;
+                    const float up = vs > 0.0f && vs < INFINITY ? power_of_two(scale_power(vs) - v_exp + kTcCodeUp) : 0.0f;
                     const __half2 up2 = __float2half2_rn(up);
                     const uint32_t mul_l = *reinterpret_cast<const uint32_t*>(&up2);
                     uint32_t mul = 0;
@@ -794,8 +797,7 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
                         low = min(min(v_low[0], v_low[1]), min(v_low[2], v_low[3]));
                         const bool some = low < 255;  // a scale that is not 0
                         *wide = some && (top < kTcScaleLow || top > kTcScaleHigh || low < top - kTcScaleSpan);
-                        // codes times 2^kTcCodeUp, weights times f = scale / 2^(exponent + 1)
-                        *unit_v = some ? power_of_two(min(max(top, kTcScaleLow), kTcScaleHigh) - 126 - kTcCodeUp) : 1.0f;
+                        *unit_v = some ? power_of_two(min(max(top, kTcScaleLow), kTcScaleHigh) - 127 - kTcCodeUp) : 1.0f;
                     }
                 }
                 named_bar_sync(2, Shape::kThreads);
