@@ -1,6 +1,6 @@
 """Where 16-bit attention over the paged 8-bit KV cache can lose a result:
 scores far from 0, large and tiny score caps, pages whose values are of very
-unlike size.  Against plain implementations in 64 bits, as in test_gpu_kv8.py,
+unlike size or NaN.  Against plain implementations in 64 bits, as in test_gpu_kv8.py,
 with tolerances that depend on what a row sees alone."""
 
 import math
@@ -243,3 +243,39 @@ def test_foreign_value_scales(ctx):
         # exact products by a power of two, until fp32's subnormal numbers: 2^-100 is not near them
         near(out.double() / f, good.double(), good.double().abs() * 2.0 ** -7 + 2.0 ** -9 * good.double().abs().max(), f"{f}")
         near(l2, lse.double(), torch.full_like(lse, 1e-4).double(), f"lse, {f}")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads", [(4, 2, 64), (8, 2, 128), (4, 2, 256)])
+@pytest.mark.parametrize("cap", [0.0, 25.0, 300.0])
+def test_non_finite_values(ctx, heads, dtype, cap):
+    """A NaN or an infinity among the values makes the outputs that see its page NaN; the weights, and so lse, are the
+    keys' and the query's alone, in every form and type.  Other rows and heads are as they would be without it."""
+    n = 260
+    c = Cache(ctx, heads, dtype, [n])
+    g = torch.Generator("cuda").manual_seed(28)
+    k, v = c.random(n, g), c.random(n, g)
+    v[100, 1, 5], v[101, 1, 9] = math.nan, -math.inf  # page 3, the second KV head
+    c.append([(k, v)])
+    q = c.queries(n, g)
+    second = torch.arange(c.h, device="cuda") >= c.h // 2
+    for window in (0, 20, 1):
+        at = torch.arange(n, device="cuda")
+        sees = (at >= 96) & (at <= 127 + window - 1 if window else True)
+        bad = sees[:, None] & second
+        ro, rl, to, tl = exact(c, 0, q, range(n), window, 0, cap, uses_tc(c, n))
+        clean = Cache(ctx, heads, dtype, [n])
+        clean.append([(k, v.nan_to_num(0, 0, 0))])
+        want, _, tol, _ = exact(clean, 0, q, range(n), window, 0, cap, uses_tc(c, n))
+        for few in (False, True):
+            rows = slice(n - 20, n) if few else slice(0, n)
+            out, lse = c.prefill(q[rows], [20 if few else n], window, cap=cap)
+            assert torch.equal(torch.isnan(out).all(2), bad[rows]) and torch.equal(torch.isnan(out).any(2), bad[rows])
+            near(lse, rl[rows], tl[rows], f"lse, window {window}")
+            ok = ~bad[rows]
+            near(out[ok], want[rows][ok], tol[rows][ok], f"out, window {window}")
+        for row in (n - 1, 130, 95):
+            out, lse = c.decode(q[row:row + 1], window, cap=cap, lens=[row + 1])
+            assert torch.equal(torch.isnan(out).all(2)[0], bad[row]) and torch.equal(torch.isnan(out).any(2)[0], bad[row])
+            near(lse, rl[row:row + 1], tl[row:row + 1], f"lse of the token, window {window}")
+    assert status(ctx) == 0

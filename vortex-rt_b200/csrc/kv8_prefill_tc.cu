@@ -27,8 +27,10 @@
 // rounded once.  So how large the values are that a row does not see, or hardly
 // weighs, costs its own no bit.  The sum of weights is kept by page in fp32 and
 // divided by f again, one FMA for 32 keys.  Pages whose value scales lie further
-// apart than 2^28, or close to fp32's ends, take the form that follows below:
-// scores and products of a row on its thread's fp32 pipes, O still in TMEM.
+// apart than 2^28, or close to fp32's ends, and pages with a NaN among their
+// values, which must reach the outputs that see them but no weight and no lse,
+// take the form that follows below: scores and products of a row on its
+// thread's fp32 pipes, O still in TMEM.
 // The running maximum moves only when it grows by more than kTcSlack (base 2):
 // weights are then up to 2^(kTcLift + kTcSlack), with f within fp16, and O is seldom
 // rescaled (a rescale waits for the tensor cores: 2500 cycles).  Beyond kTcFar
@@ -507,26 +509,25 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
             const TcMeta* mt = meta + (j / SUB & 3) * PG + j % SUB * 2;
             float a0 = mt[0].k_scale * factor, a1 = mt[1].k_scale * factor, b0 = mt[0].v_log, b1 = mt[1].v_log;
             // a score times a plus b is the exponent of its weight times the value scale, inv takes that back for the
-            // sum; a NaN (of a page's scales, or of the query in `factor`) reaches the sum, and so the row, through inv
+            // sum; a NaN (of a page's keys, or of the query in `factor`) reaches the sum, and so the row, through inv
             float i0v = mt[0].v_inv, i1v = mt[1].v_inv;
             const int i0p = static_cast<int>(j0) + 2 * j;
             const bool whole = (i0p + 1 < whole_a || (i0p >= whole_b && i0p + 1 < whole_c)) && !*missing;
             tmem_arrived(va, vb);
             if (!whole) {
                 // Takes a page's scores to what the row sees: the rest is -inf, so the factor is kept above 0, and a NaN
-                // scale of a page that the row does not see is left out.
-                auto mask = [&](int c, uint32_t(&v)[32], float& a, float& b, float& inv) {
+                // key scale of a page that the row does not see is left out.
+                auto mask = [&](int c, uint32_t(&v)[32], float& a, float& inv) {
                     const int t0 = static_cast<int>(span.page(j0 + 2 * j + c) * kKv8Page);
                     const uint32_t see = mt[c].there ? visible(t0) : 0u;
-                    const bool bad = !(a < INFINITY) || !(b < INFINITY);
+                    const bool bad = !(a < INFINITY);
                     a = bad ? 1.0f : fmaxf(a, 1e-37f);
-                    b = bad ? 0.0f : b;
                     inv = bad ? (see ? NAN : 1.0f) : inv;
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[i] = see >> i & 1 ? v[i] : 0xff800000u;
                 };
-                mask(0, va, a0, b0, i0v);
-                mask(1, vb, a1, b1, i1v);
+                mask(0, va, a0, i0v);
+                mask(1, vb, a1, i1v);
             } else {
                 i0v = a0 < INFINITY ? i0v : NAN;
                 i1v = a1 < INFINITY ? i1v : NAN;
@@ -717,8 +718,8 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
                             e.k_scale = ks;
                             if (vs != 0.0f) {
                                 const float f = scale_rest(vs);
-                                e.v_log = vs < INFINITY ? log2f(f) : NAN;
-                                e.v_inv = vs < INFINITY ? 1.0f / f : NAN;
+                                e.v_log = log2f(f);
+                                e.v_inv = 1.0f / f;
                             }
                         }
                         meta[(j & 3) * PG + c0] = e;
@@ -729,8 +730,8 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
                         store_codes(at + to + i * step, at + (to ^ 16u) + i * step, r[i]);
                     }
                 } else {
-                    // the power of two that the codes of page `lane` are stored times; 0 for a page of zeros or NaN
-                    const float up = vs > 0.0f && vs < INFINITY ? power_of_two(scale_power(vs) - v_exp + kTcCodeUp) : 0.0f;
+                    // the power of two that the codes of page `lane` are stored times; 0 for a page of zeros
+                    const float up = vs > 0.0f ? power_of_two(scale_power(vs) - v_exp + kTcCodeUp) : 0.0f;
                     const __half2 up2 = __float2half2_rn(up);
                     const uint32_t mul_l = *reinterpret_cast<const uint32_t*>(&up2);
                     uint32_t mul = 0;
@@ -784,7 +785,7 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
                     for (uint32_t i = j0 + c0; i < j1; i += 128) {
                         const int id = kv8_page(p.a.c, seq, span.page(i), p.a.status);
                         const float v = id < 0 ? 0.0f : p.a.c.v_scale[static_cast<uint64_t>(id) * p.a.c.kv + g];
-                        if (v == 0.0f || !(v < INFINITY)) continue;
+                        if (v == 0.0f) continue;
                         top = max(top, scale_exponent(v));
                         low = min(low, v > 0.0f ? scale_exponent(v) : 0);
                     }
