@@ -1,6 +1,6 @@
 """Where 16-bit attention over the paged 8-bit KV cache can lose a result:
 scores far from 0, large and tiny score caps, pages whose values are of very
-unlike size or NaN.  Against plain implementations in 64 bits, as in test_gpu_kv8.py,
+unlike size or NaN, long histories.  Against plain implementations in 64 bits, as in test_gpu_kv8.py,
 with tolerances that depend on what a row sees alone."""
 
 import math
@@ -56,8 +56,9 @@ def exact(c, i, q, pos, window=0, prefix=0, cap=0.0, tc=False):
     tol = tol + (2.0 ** -28 if tc else 2.0 ** -39) * cut
     # twice a weight's error is exp(2 ds) - 1 <= 4 ds only for ds <= 1/2; where scores are so large that theirs is
     # beyond 1/4, any weights are right that are none below 0 and sum to 1: an output lies among the values seen
-    most = torch.where(see[:, :, None, None], vz.abs()[None], 0.0).amax(1) * (1 + 4 * HALF[c.dtype])
-    tol = torch.where((ds > 0.25)[..., None], out.abs() + most, tol)
+    if (ds > 0.25).any():
+        most = torch.where(see[:, :, None, None], vz.abs()[None], 0.0).amax(1) * (1 + 4 * HALF[c.dtype])
+        tol = torch.where((ds > 0.25)[..., None], out.abs() + most, tol)
     return out, lse, tol, ds + sums + lse.abs().nan_to_num(0, 0, 0) * U
 
 
@@ -278,4 +279,54 @@ def test_non_finite_values(ctx, heads, dtype, cap):
             out, lse = c.decode(q[row:row + 1], window, cap=cap, lens=[row + 1])
             assert torch.equal(torch.isnan(out).all(2)[0], bad[row]) and torch.equal(torch.isnan(out).any(2)[0], bad[row])
             near(lse, rl[row:row + 1], tl[row:row + 1], f"lse of the token, window {window}")
+    assert status(ctx) == 0
+
+
+ALL_ONE = 70000  # an upper bound of new rows from which a history is not split
+
+
+@pytest.mark.parametrize("heads,dtype,m", [((8, 1, 64), "f16", 64), ((2, 1, 128), "f16", 40), ((1, 1, 256), "f16", 40),
+                                           ((2, 1, 128), "bf16", 40)])
+def test_long_sums(ctx, heads, dtype, m):
+    """Sums over 300,000 keys in one piece stay in the middle.
+
+    Positive values and nearly equal weights, so that a sum that is cut at every addition falls behind all the time:
+    by a step U at most in each of a run's 16,384 / 16 = 1024 additions.  Runs, and the sums of weights by page, are
+    joined by rounding additions, half a step each.  What is rounded to 16 bits, weights and outputs, is right on
+    average: its mean over the outputs is below a twentieth of the half step that each may be off by."""
+    n = 300000
+    c = Cache(ctx, heads, dtype, [n])
+    g = torch.Generator("cuda").manual_seed(29)
+    for i in range(0, n, 50000):
+        c.append([(c.random(50000, g), (1 + torch.rand((50000, c.kv, c.hd), generator=g, device="cuda")).to(TYPES[dtype]))])
+    q = c.queries(m, g, 0.02)
+    out, lse = c.prefill(q, [m], max_new=ALL_ONE)
+    k, v = c.values(0)
+    s = torch.einsum("mhd,td->mht", q.double(), k[:, 0]) * c.hd ** -0.5
+    t = torch.arange(n, device="cuda")
+    s.masked_fill_(t > torch.arange(n - m, n, device="cuda")[:, None, None], -math.inf)
+    ref = torch.einsum("mht,td->mhd", torch.softmax(s, 2), v[:, 0])
+    off = (out.double() - ref) / ref
+    sums = 1024 * U + n / PAGE * U / 2
+    assert off.mean().abs() <= sums + (HALF[dtype] + 2.0 ** -11) / 20, f"{off.mean():.3g}"
+    assert off.abs().max() <= sums + HALF[dtype] + 2.0 ** -11, f"{off.abs().max():.3g}"
+    near(lse, torch.logsumexp(s, 2), torch.full_like(lse, sums + 64 * U).double() + (c.hd + 8) * U, "lse")
+
+
+@pytest.mark.parametrize("heads,dtype", [((8, 1, 64), "f16"), ((6, 2, 128), "bf16"), ((2, 1, 256), "f16")])
+@pytest.mark.parametrize("n", [16384, 16385, 16448, 33000, 49153])
+def test_long_runs(ctx, heads, dtype, n):
+    """Histories of whole and broken runs whose scores rise and fall from run to run."""
+    m = 70
+    c = Cache(ctx, heads, dtype, [ALL_ONE])
+    g = torch.Generator("cuda").manual_seed(30)
+    k, v = c.random(n, g), c.random(n, g)
+    size = 1 + 2 * torch.sin(torch.arange(n, device="cuda") / 6000)[:, None, None]
+    c.append([((k.float() * size).to(TYPES[dtype]), v)])
+    q = c.queries(m, g, 3.0)
+    for window, prefix, cap in ((0, 0, 0.0), (n - 20, 0, 30.0), (9000, 12000, 0.0)):
+        out, lse = c.prefill(q, [m], window, [prefix] if prefix else None, cap, max_new=ALL_ONE)
+        ro, rl, to, tl = exact(c, 0, q, range(n - m, n), window, prefix, cap, True)
+        near(out, ro, to, f"window {window}, prefix {prefix}, cap {cap}")
+        near(lse, rl, tl, f"lse, window {window}, prefix {prefix}, cap {cap}")
     assert status(ctx) == 0

@@ -38,6 +38,13 @@
 // is a rounded score, by whole numbers: there scores are rounded first.  What falls
 // under fp16's smallest step is 2^-28 of a row's largest weight, times values that
 // the row sees, each its own: far below half a step of a 16-bit output.
+// O: the tensor core cuts the sum that it adds 16 keys to, always towards 0, by
+// some 2^-24 of it: 1e-4 after 32,768 keys and 4e-4 after 131,072 (measured; an
+// f16 output is rounded by 4.9e-4 at most).  So every kTcRun key tiles O is added
+// to a sum in fp32 in the thread's local memory, by rounding additions, and
+// starts again from 0.  A form of its own (RUNS) for calls that may see so many
+// keys: its code made 8192 tokens 757 us instead of 740, 4x2048 capped 99
+// instead of 94.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -50,6 +57,7 @@
 namespace vrt {
 
 constexpr float kTcSlack = 11.5f, kTcLift = 3.5f;
+constexpr int kTcRun = 256;  // key tiles of a run: 16,384 keys
 constexpr float kTcFar = 1048576.0f;  // scores (base 2) whose fp32 step is an eighth
 
 // Value scales by the exponent field of their fp32: the largest of a CTA's
@@ -285,8 +293,8 @@ __device__ __forceinline__ void tmem_arrived(uint32_t (&a)[32], uint32_t (&b)[32
     for (int c = 0; c < 32; ++c) asm volatile("" : "+r"(a[c]), "+r"(b[c]));
 }
 
-// CAP: 0 plain scores, 1 capped up to kKv8FastCap, 2 capped above it (tanhf)
-template <typename T, int HD, int CAP>
+// CAP: 0 plain scores, 1 capped up to kKv8FastCap, 2 capped above it (tanhf).  RUNS: more than kTcRun key tiles.
+template <typename T, int HD, int CAP, bool RUNS>
 __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kernel(const Kv8Split p) {
     using Shape = TcShape<HD>;
     constexpr int MT = Shape::MT, KT = Shape::KT, KB = Shape::KB, SUB = Shape::SUB, PG = Shape::PG, ST = Shape::kStages;
@@ -430,6 +438,7 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
             named_bar_sync(2, Shape::kThreads);  // the value scales have been looked through
             slow = *wide;
         }
+        float kept[HD], kept_mx = -INFINITY;  // O of the runs before, weighed from kept_mx
         if (__builtin_expect(slow, 0)) {
             const uint32_t at_o = tmem + lanes + Shape::kOCol + t * HD;
             const int pages = min(2 * mine, static_cast<int>(j1 - j0));
@@ -573,6 +582,27 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
                     tmem_wait_st();
                 }
             }
+            if (RUNS && j > 0 && j % kTcRun == 0) {
+                uint64_t* added = j + 1 < mine ? s_full + 2 * t + ((j + 1) & 1) : o_last + 2 * t;
+                ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded(added, j + 1 < mine ? ((j + 1) >> 1) & 1 : 0));
+                if (!ok) break;
+                tc_fence_after();
+                const float f = kept_mx == -INFINITY ? 0.0f : ex2(kept_mx - mx);
+                kept_mx = mx;
+#pragma unroll 1
+                for (int d = 0; d < HD; d += 16) {
+                    uint32_t o[16];
+                    const uint32_t at_o = tmem + lanes + Shape::kOCol + t * HD + d;
+                    tmem_ld16(at_o, o);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        kept[d + e] = j == kTcRun ? __uint_as_float(o[e]) : fmaf(kept[d + e], f, __uint_as_float(o[e]));
+                        o[e] = 0u;
+                    }
+                    tmem_st16(at_o, o);
+                }
+                tmem_wait_st();
+            }
             const float seen = mx == -INFINITY ? 0.0f : mx, base = kTcLift - seen;
             // kHidden: scores of -inf among them, which a tanh would make finite; kFar: scores beyond kTcFar
             auto weigh = [&](int c, const uint32_t(&v)[32], float a, float b, float inv, auto kHidden, auto kFar) {
@@ -648,10 +678,16 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
         const float mul = used == 1 ? (sum == 0.0f ? 0.0f : ref / sum) : ref;
         T* out = static_cast<T*>(p.a.out) + at * p.a.out_stride + static_cast<uint64_t>(h) * HD;
         const uint64_t prow = ((static_cast<uint64_t>(seq) * p.a.max_new + i0 + token) * p.a.H + h) * p.splits + split;
+        const bool more = RUNS && !slow && mine > kTcRun;
+        const float f_kept = kept_mx == -INFINITY ? 0.0f : ex2(kept_mx - mx);
 #pragma unroll 2
         for (int d = 0; d < HD; d += 16) {
             uint32_t v[16] = {};
             if (mine > 0) tmem_ld16(tmem + lanes + Shape::kOCol + t * HD + d, v);
+            if (more) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(fmaf(kept[d + e], f_kept, __uint_as_float(v[e])));
+            }
             if (live && used == 1) {
                 uint32_t x[8];
 #pragma unroll
@@ -882,7 +918,7 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
 
 // -------------------------------------------------------------------- host
 
-template <typename T, int HD, int CAP>
+template <typename T, int HD, int CAP, bool RUNS>
 static cudaError_t tc_launch(const Kv8Split& p, cudaStream_t s) {
     using Shape = TcShape<HD>;
     static std::mutex mu;
@@ -894,30 +930,32 @@ static cudaError_t tc_launch(const Kv8Split& p, cudaStream_t s) {
         std::lock_guard<std::mutex> lock(mu);
         const uint64_t bit = dev < 64 ? 1ull << dev : 0ull;
         if (!(done & bit)) {
-            e = cudaFuncSetAttribute(kv8_prefill_tc_kernel<T, HD, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kBytes);
+            e = cudaFuncSetAttribute(kv8_prefill_tc_kernel<T, HD, CAP, RUNS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kBytes);
             if (e != cudaSuccess) return e;
             done |= bit;
         }
     }
     const dim3 grid((p.a.max_new + p.tile - 1) / p.tile * p.a.c.kv, 1, p.a.count * p.splits);
-    e = launch(kv8_prefill_tc_kernel<T, HD, CAP>, grid, dim3(Shape::kThreads), Shape::kBytes, s, false, p);
+    e = launch(kv8_prefill_tc_kernel<T, HD, CAP, RUNS>, grid, dim3(Shape::kThreads), Shape::kBytes, s, false, p);
     if (e != cudaSuccess || p.splits == 1) return e;
     return kv8_join(p, HD, p.a.dtype, s);
 }
 
 uint32_t kv8_prefill_tc_rows(uint32_t hd) { return hd == 256 ? 128u : 256u; }
 
+template <typename T, int HD>
+static cudaError_t tc_form(const Kv8Split& p, cudaStream_t s) {
+    const bool runs = p.chunk > 2 * kTcRun;  // two pages a key tile
+    if (p.a.softcap > kKv8FastCap) return tc_launch<T, HD, 2, true>(p, s);
+    if (p.a.softcap > 0.0f) return runs ? tc_launch<T, HD, 1, true>(p, s) : tc_launch<T, HD, 1, false>(p, s);
+    return runs ? tc_launch<T, HD, 0, true>(p, s) : tc_launch<T, HD, 0, false>(p, s);
+}
+
 cudaError_t kv8_prefill_tc(const Kv8Split& p, uint32_t hd, cudaStream_t s) {
-    const int cap = p.a.softcap > kKv8FastCap ? 2 : p.a.softcap > 0.0f ? 1 : 0;
-#define VRT_TC(HD)                                                                                                  \
-    if (hd == HD) {                                                                                                 \
-        if (p.a.dtype == VRT_F16) {                                                                                 \
-            return cap == 2 ? tc_launch<__half, HD, 2>(p, s) : cap ? tc_launch<__half, HD, 1>(p, s) : tc_launch<__half, HD, 0>(p, s); \
-        }                                                                                                           \
-        if (p.a.dtype == VRT_BF16) {                                                                                \
-            return cap == 2 ? tc_launch<__nv_bfloat16, HD, 2>(p, s)                                                 \
-                            : cap ? tc_launch<__nv_bfloat16, HD, 1>(p, s) : tc_launch<__nv_bfloat16, HD, 0>(p, s);  \
-        }                                                                                                           \
+#define VRT_TC(HD)                                                              \
+    if (hd == HD) {                                                             \
+        if (p.a.dtype == VRT_F16) return tc_form<__half, HD>(p, s);             \
+        if (p.a.dtype == VRT_BF16) return tc_form<__nv_bfloat16, HD>(p, s);     \
     }
     VRT_TC(64) VRT_TC(128) VRT_TC(256)
 #undef VRT_TC
