@@ -2616,7 +2616,8 @@ static int batch_create(vrt_model* m, uint32_t max_seqs, uint32_t max_positions,
             sizes.push_back(S * m->KVl * kKv8Page * hd * 4);
             continue;
         }
-        const uint32_t cap = m->layers[l].global ? max_positions : std::min(c.sliding_window, max_positions);
+        const bool windowed = !m->layers[l].global && c.sliding_window;  // no window: all positions, as on global layers
+        const uint32_t cap = windowed ? std::min(c.sliding_window, max_positions) : max_positions;
         b->cap.push_back(cap);
         sizes.push_back(S * m->KVl * cap * hd * 4);  // K
         sizes.push_back(S * m->KVl * cap * hd * 4);  // V
