@@ -1817,7 +1817,8 @@ static uint64_t kv8_ring_pages(uint32_t window) { return (static_cast<uint64_t>(
 // Pages of one sequence in layer l's 8-bit cache.
 static uint64_t batch_kv8_pages(const vrt_model* m, uint32_t l, uint32_t positions) {
     const uint64_t pps = (static_cast<uint64_t>(positions) + kKv8Page - 1) / kKv8Page;
-    return m->layers[l].global ? pps : std::min(pps, kv8_ring_pages(m->cfg.sliding_window));
+    const bool windowed = !m->layers[l].global && m->cfg.sliding_window;
+    return windowed ? std::min(pps, kv8_ring_pages(m->cfg.sliding_window)) : pps;
 }
 
 // Workspace for every step and prefill slice that the batch may run.
@@ -2699,7 +2700,7 @@ static int batch_create(vrt_model* m, uint32_t max_seqs, uint32_t max_positions,
         std::vector<int32_t> host(S * pps);
         for (uint32_t l = 0; l < c.block_count; ++l) b->kv8_layer[l].table = tables[m->layers[l].global ? 1 : 0];
         for (int global = 0; global < 2; ++global) {
-            const uint64_t ring = global ? pps : std::min<uint64_t>(pps, kv8_ring_pages(c.sliding_window));
+            const uint64_t ring = global || !c.sliding_window ? pps : std::min<uint64_t>(pps, kv8_ring_pages(c.sliding_window));
             for (uint64_t q = 0; q < S; ++q)
                 for (uint64_t j = 0; j < pps; ++j) host[q * pps + j] = static_cast<int32_t>(q * ring + j % ring);
             VRT_CUDA(cudaMemcpyAsync(tables[global], host.data(), host.size() * 4, cudaMemcpyHostToDevice, m->ctx->stream));
