@@ -1,6 +1,7 @@
 """Where 16-bit attention over the paged 8-bit KV cache can lose a result:
 scores far from 0, large and tiny score caps, pages whose values are of very
-unlike size or NaN, long histories.  Against plain implementations in 64 bits, as in test_gpu_kv8.py,
+unlike size or NaN, long histories, a capacity far above the
+lengths.  Against plain implementations in 64 bits, as in test_gpu_kv8.py,
 with tolerances that depend on what a row sees alone."""
 
 import math
@@ -329,4 +330,39 @@ def test_long_runs(ctx, heads, dtype, n):
         ro, rl, to, tl = exact(c, 0, q, range(n - m, n), window, prefix, cap, True)
         near(out, ro, to, f"window {window}, prefix {prefix}, cap {cap}")
         near(lse, rl, tl, f"lse, window {window}, prefix {prefix}, cap {cap}")
+    assert status(ctx) == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens", [[1000], [1024, 1, 0, 517]])
+def test_capacity_far_above_lengths(ctx, dtype, lens):
+    """Full-width heads with a table and max_len of 32,768 positions, as a batch gives them, and a few short sequences."""
+    c = Cache(ctx, (32, 16, 128), dtype, [max(1, n) for n in lens], pages=200)
+    wide = torch.full((len(lens), 1024), -1, dtype=torch.int32, device="cuda")
+    wide[:, :c.pps] = c.table
+    c.table, c.pps = wide, 1024
+    c.c.s.pages_per_seq, c.c.s.d_table = 1024, wide.data_ptr()
+    g = torch.Generator("cuda").manual_seed(31)
+    c.append([(c.random(n, g), c.random(n, g)) for n in lens])
+    new = [min(n, 33) for n in lens]
+    for window, prefix in ((0, 0), (200, 0), (200, 4)):
+        pre = [min(n, prefix) for n in lens] if prefix else None
+        q = c.queries(len(lens), g)
+        out, lse = c.decode(q, window, pre, max_len=32768)
+        for i, n in enumerate(lens):
+            if n:
+                ro, rl, to, tl = exact(c, i, q[i:i + 1], [n - 1], window, pre[i] if pre else 0)
+                near(out[i:i + 1], ro, to, f"token of {n}")
+                near(lse[i:i + 1], rl, tl, f"lse of the token of {n}")
+            else:
+                assert (out[i] == 0).all() and torch.isneginf(lse[i]).all()
+        q = c.queries(sum(new), g)
+        out, lse = c.prefill(q, new, window, pre, max_len=32768)
+        r = 0
+        for i, (n, m) in enumerate(zip(lens, new)):
+            if m:
+                ro, rl, to, tl = exact(c, i, q[r:r + m], range(n - m, n), window, pre[i] if pre else 0, tc=uses_tc(c, max(new)))
+                near(out[r:r + m], ro, to, f"chunk of {n}")
+                near(lse[r:r + m], rl, tl, f"lse of the chunk of {n}")
+            r += m
     assert status(ctx) == 0
