@@ -27,10 +27,11 @@
 // rounded once.  So how large the values are that a row does not see, or hardly
 // weighs, costs its own no bit.  The sum of weights is kept by page in fp32 and
 // divided by f again, one FMA for 32 keys.  Pages whose value scales lie further
-// apart than 2^28, or close to fp32's ends, and pages with a NaN among their
-// values, which must reach the outputs that see them but no weight and no lse,
-// take the form that follows below: scores and products of a row on its
-// thread's fp32 pipes, O still in TMEM.
+// apart than 2^28, or close to fp32's ends, take the form that follows below:
+// scores and products of a row on its thread's fp32 pipes, O still in TMEM
+// (8192 tokens in such a cache: 39 ms instead of 0.74).  A page with a NaN among
+// its values counts as zeros; the outputs that see it are made NaN in the end,
+// and no weight and no lse.
 // The running maximum moves only when it grows by more than kTcSlack (base 2):
 // weights are then up to 2^(kTcLift + kTcSlack), with f within fp16, and O is seldom
 // rescaled (a rescale waits for the tensor cores: 2500 cycles).  Beyond kTcFar
@@ -322,6 +323,7 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
     volatile int* wide = reinterpret_cast<volatile int*>(v_low + 4);  // scales too far apart for fp16 codes
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_low + 5);
     volatile int* missing = reinterpret_cast<volatile int*>(tmem_slot + 1);  // a page was not in the pool
+    volatile int* poisoned = missing + 1;                                    // a page has a NaN among its values
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t R = p.a.H / p.a.c.kv, g = blockIdx.x % p.a.c.kv;
@@ -365,6 +367,7 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
         }
         for (int t = 0; t < 2; ++t) mbar_init(drained + t, 1);
         *missing = 0;
+        *poisoned = 0;
         *wide = 0;
         fence_mbar_init();
     }
@@ -437,6 +440,16 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
         if (J > 0) {
             named_bar_sync(2, Shape::kThreads);  // the value scales have been looked through
             slow = *wide;
+        }
+        bool poison = false;  // the row sees a page with a NaN among its values
+        if (mine > 0 && *poisoned) {
+#pragma unroll 1
+            for (uint32_t i = j0; i < min(j0 + 2 * mine, j1); ++i) {
+                const uint32_t page = span.page(i);
+                const int id = kv8_page(p.a.c, seq, page, p.a.status);
+                const float v = id < 0 ? 0.0f : p.a.c.v_scale[static_cast<uint64_t>(id) * p.a.c.kv + g];
+                if (v != v && visible(static_cast<int>(page * kKv8Page))) poison = true;
+            }
         }
         float kept[HD], kept_mx = -INFINITY;  // O of the runs before, weighed from kept_mx
         if (__builtin_expect(slow, 0)) {
@@ -675,7 +688,8 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
         }
         if (mx == -INFINITY && sum < INFINITY) sum = 0.0f;  // nothing seen: what ex2_fma makes of -inf
         const float ref = mine > 0 ? (slow ? 1.0f : *unit_v) : 0.0f;
-        const float mul = used == 1 ? (sum == 0.0f ? 0.0f : ref / sum) : ref;
+        float mul = used == 1 ? (sum == 0.0f ? 0.0f : ref / sum) : ref;
+        if (poison) mul = NAN;
         T* out = static_cast<T*>(p.a.out) + at * p.a.out_stride + static_cast<uint64_t>(h) * HD;
         const uint64_t prow = ((static_cast<uint64_t>(seq) * p.a.max_new + i0 + token) * p.a.H + h) * p.splits + split;
         const bool more = RUNS && !slow && mine > kTcRun;
@@ -752,7 +766,7 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
                         TcMeta e{0.0f, 0.0f, 1.0f, id >= 0};
                         if (e.there) {
                             e.k_scale = ks;
-                            if (vs != 0.0f) {
+                            if (vs != 0.0f && vs == vs) {
                                 const float f = scale_rest(vs);
                                 e.v_log = log2f(f);
                                 e.v_inv = 1.0f / f;
@@ -766,7 +780,7 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
                         store_codes(at + to + i * step, at + (to ^ 16u) + i * step, r[i]);
                     }
                 } else {
-                    // the power of two that the codes of page `lane` are stored times; 0 for a page of zeros
+                    // the power of two that the codes of page `lane` are stored times; 0 for a page of zeros or NaN
                     const float up = vs > 0.0f ? power_of_two(scale_power(vs) - v_exp + kTcCodeUp) : 0.0f;
                     const __half2 up2 = __float2half2_rn(up);
                     const uint32_t mul_l = *reinterpret_cast<const uint32_t*>(&up2);
@@ -821,7 +835,8 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
                     for (uint32_t i = j0 + c0; i < j1; i += 128) {
                         const int id = kv8_page(p.a.c, seq, span.page(i), p.a.status);
                         const float v = id < 0 ? 0.0f : p.a.c.v_scale[static_cast<uint64_t>(id) * p.a.c.kv + g];
-                        if (v == 0.0f) continue;
+                        if (v != v) *poisoned = 1;
+                        if (v == 0.0f || v != v) continue;
                         top = max(top, scale_exponent(v));
                         low = min(low, v > 0.0f ? scale_exponent(v) : 0);
                     }
