@@ -1,7 +1,7 @@
 """Where 16-bit attention over the paged 8-bit KV cache can lose a result:
 scores far from 0, large and tiny score caps, pages whose values are of very
-unlike size or NaN, long histories, a capacity far above the
-lengths.  Against plain implementations in 64 bits, as in test_gpu_kv8.py,
+unlike size or NaN, long histories, values near fp32's end, a
+capacity far above the lengths.  Against plain implementations in 64 bits, as in test_gpu_kv8.py,
 with tolerances that depend on what a row sees alone."""
 
 import math
@@ -331,6 +331,30 @@ def test_long_runs(ctx, heads, dtype, n):
         near(out, ro, to, f"window {window}, prefix {prefix}, cap {cap}")
         near(lse, rl, tl, f"lse, window {window}, prefix {prefix}, cap {cap}")
     assert status(ctx) == 0
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("heads", [(8, 2, 64), (8, 2, 128), (4, 1, 256)])
+@pytest.mark.parametrize("n,m", [(300, 150), (2500, 33), (6000, 3)])
+def test_values_near_the_end(ctx, heads, dtype, n, m):
+    """Values of 1e36: a sum of them with weights up to 1 is within fp32, with weights held larger it is not."""
+    c = Cache(ctx, heads, dtype, [n])
+    g = torch.Generator("cuda").manual_seed(32)
+    v = (1e36 * torch.randn((n, c.kv, c.hd), generator=g, device="cuda")).to(TYPES[dtype])
+    v[64:96] *= 2.0 ** -60  # the tcgen05 form's fp32 pipes too, where the page is walked
+    c.append([(c.random(n, g), v)])
+    q = c.queries(m, g)
+    for window, cap in ((0, 0.0), (40, 20.0)):
+        for few in (False, True):
+            rows = slice(m - min(m, 20), m) if few else slice(0, m)
+            out, lse = c.prefill(q[rows], [rows.stop - rows.start], window, cap=cap)
+            ro, rl, to, tl = exact(c, 0, q[rows], range(n - m, n)[rows], window, 0, cap, uses_tc(c, rows.stop - rows.start))
+            near(out, ro, to, f"prompt, window {window}")
+            near(lse, rl, tl, f"lse of the prompt, window {window}")
+        out, lse = c.decode(q[m - 1:], window, cap=cap)
+        ro, rl, to, tl = exact(c, 0, q[m - 1:], [n - 1], window, 0, cap)
+        near(out, ro, to, f"token, window {window}")
+        near(lse, rl, tl, f"lse of the token, window {window}")
 
 
 @pytest.mark.parametrize("dtype", TYPES)

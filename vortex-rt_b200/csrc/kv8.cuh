@@ -72,8 +72,8 @@ struct Kv8Split {
     uint32_t tile;    // query tokens that see their pages together
     uint32_t chunk;   // pages of one split at most
     uint32_t splits;  // of the longest sequence
-    float* part;      // [count][max_new][H][splits][head_dim] unnormalised outputs
-    float* part_ml;   // [count][max_new][H][splits][2] maximum (base 2) and sum
+    float* part;      // [count][max_new][H][splits][head_dim] outputs of a split alone
+    float* part_ml;   // [count][max_new][H][splits][2] its maximum (base 2) and sum of weights
 };
 
 // Pool index of page `page` of sequence `seq`, -1 (and the status bit) when
@@ -222,6 +222,17 @@ __device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
     const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&b), __float2half2_rn(1152.0f));
     return *reinterpret_cast<const uint32_t*>(&h);
 }
+
+// The same times 2^-kKv8Lift (exact), for values: they meet weights that are held
+// times 2^kKv8Lift, and the products are sums of at most the values' own size,
+// which fp32 holds as far as it holds the values.
+__device__ __forceinline__ uint32_t value_codes(uint32_t b) {
+    const __half2 h = __hfma2(*reinterpret_cast<const __half2*>(&b), __float2half2_rn(0x1p-14f), __float2half2_rn(-1152.0f * 0x1p-14f));
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t value_codes_lo(uint32_t w) { return value_codes(__byte_perm(w, 0x64646464u, 0x4140u)); }
+__device__ __forceinline__ uint32_t value_codes_hi(uint32_t w) { return value_codes(__byte_perm(w, 0x64646464u, 0x4342u)); }
+constexpr float kKv8Unlift = 16384.0f;  // what such a sum is multiplied by before it is divided by the weights'
 
 __device__ __forceinline__ uint32_t pack_half(__half a, __half b) {
     return static_cast<uint32_t>(__half_as_ushort(a)) | static_cast<uint32_t>(__half_as_ushort(b)) << 16;

@@ -316,8 +316,8 @@ __global__ void __launch_bounds__(kKdThreads, KdShape<HD>::kCtas) kv8_decode_ker
                 u1.x ^= 0x80808080u;
                 u1.y ^= 0x80808080u;
                 float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                const uint32_t a0 = codes_lo(u0.x), a1 = codes_lo(u1.x), a2 = codes_hi(u0.x), a3 = codes_hi(u1.x);
-                const uint32_t c0 = codes_lo(u0.y), c1 = codes_lo(u1.y), c2 = codes_hi(u0.y), c3 = codes_hi(u1.y);
+                const uint32_t a0 = value_codes_lo(u0.x), a1 = value_codes_lo(u1.x), a2 = value_codes_hi(u0.x), a3 = value_codes_hi(u1.x);
+                const uint32_t c0 = value_codes_lo(u0.y), c1 = value_codes_lo(u1.y), c2 = value_codes_hi(u0.y), c3 = value_codes_hi(u1.y);
                 if (SETS == 2) {
                     mma_f16(o, a0, a1, a2, a3, make_uint2(pl[0], pl[1]));
                     mma_f16(o, c0, c1, c2, c3, make_uint2(pl[2], pl[3]));
@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(kKdThreads, KdShape<HD>::kCtas) kv8_decode_ker
         const uint64_t row = static_cast<uint64_t>(seq) * p.a.H + g * R + r;
         float* part = p.part + (row * p.splits + split) * HD;
         T* out = static_cast<T*>(p.a.out) + static_cast<uint64_t>(seq) * p.a.out_stride + static_cast<uint64_t>(g * R + r) * HD;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const float inv = l == 0.0f ? 0.0f : kKv8Unlift / l;
         for (int d = lane; d < HD; d += 32) {
             float v = 0.0f;
 #pragma unroll
@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(kKdThreads, KdShape<HD>::kCtas) kv8_decode_ker
             if (alone) {
                 out[d] = from_f32<T>(v * inv);
             } else {
-                part[d] = v;
+                part[d] = v * inv;
             }
         }
         if (lane == 0) {

@@ -47,10 +47,17 @@ __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], const __half* p) {
 }
 
 // 16 codes -> 16 fp16
+template <bool VALUES>
 __device__ __forceinline__ void store_codes(__half* dst, uint4 u) {
     const uint32_t w[4] = {u.x ^ 0x80808080u, u.y ^ 0x80808080u, u.z ^ 0x80808080u, u.w ^ 0x80808080u};
-    reinterpret_cast<uint4*>(dst)[0] = make_uint4(codes_lo(w[0]), codes_hi(w[0]), codes_lo(w[1]), codes_hi(w[1]));
-    reinterpret_cast<uint4*>(dst)[1] = make_uint4(codes_lo(w[2]), codes_hi(w[2]), codes_lo(w[3]), codes_hi(w[3]));
+    uint32_t h[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        h[2 * i] = VALUES ? value_codes_lo(w[i]) : codes_lo(w[i]);
+        h[2 * i + 1] = VALUES ? value_codes_hi(w[i]) : codes_hi(w[i]);
+    }
+    reinterpret_cast<uint4*>(dst)[0] = make_uint4(h[0], h[1], h[2], h[3]);
+    reinterpret_cast<uint4*>(dst)[1] = make_uint4(h[4], h[5], h[6], h[7]);
 }
 
 template <typename T, int HD, int TERMS>
@@ -159,8 +166,8 @@ __global__ void __launch_bounds__(kKpThreads) kv8_prefill_kernel(const Kv8Split 
 #pragma unroll
         for (int i = 0; i < C; ++i) {
             const int c = tid + i * kKpThreads;
-            store_codes(ks + c / (HD / 16) * Shape::kK + c % (HD / 16) * 16, kr[i]);
-            store_codes(vs + c / 2 * Shape::kV + c % 2 * 16, vr[i]);
+            store_codes<false>(ks + c / (HD / 16) * Shape::kK + c % (HD / 16) * 16, kr[i]);
+            store_codes<true>(vs + c / 2 * Shape::kV + c % 2 * 16, vr[i]);
         }
         const float k_now = k_scale, v_now = v_scale;
         const bool here = there;
@@ -291,8 +298,8 @@ __global__ void __launch_bounds__(kKpThreads) kv8_prefill_kernel(const Kv8Split 
         sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
         const uint32_t r = 16 * warp + g8 + 8 * i, token = r / R, h = g * R + r % R;
         if (token >= tokens) continue;
+        const float l = sum[i], inv = l == 0.0f ? 0.0f : kKv8Unlift / l;
         if (used == 1) {
-            const float l = sum[i], inv = l == 0.0f ? 0.0f : 1.0f / l;
             const uint64_t row = static_cast<uint64_t>(r0 + i0 + token);
             T* out = static_cast<T*>(p.a.out) + row * p.a.out_stride + static_cast<uint64_t>(h) * HD;
 #pragma unroll
@@ -306,12 +313,12 @@ __global__ void __launch_bounds__(kKpThreads) kv8_prefill_kernel(const Kv8Split 
             float* part = p.part + row * HD;
 #pragma unroll
             for (int d = 0; d < NT; ++d) {
-                part[8 * d + 2 * t4] = acc[d][2 * i];
-                part[8 * d + 2 * t4 + 1] = acc[d][2 * i + 1];
+                part[8 * d + 2 * t4] = acc[d][2 * i] * inv;
+                part[8 * d + 2 * t4 + 1] = acc[d][2 * i + 1] * inv;
             }
             if (t4 == 0) {
                 p.part_ml[row * 2] = kv8_base(mx[i]);
-                p.part_ml[row * 2 + 1] = sum[i];
+                p.part_ml[row * 2 + 1] = l;
             }
         }
     }
@@ -355,22 +362,22 @@ __global__ void __launch_bounds__(kKjThreads) kv8_join_few_kernel(const Kv8Split
     for (uint32_t s = 0; s < kKjFew; ++s) {
         const bool there = s < used;
         const float ms = there ? ml[2 * s] : -INFINITY;
-        f[s] = ms == -INFINITY ? 1.0f : ex2(ms - m);
-        l += there ? ml[2 * s + 1] * f[s] : 0.0f;
+        f[s] = there ? ml[2 * s + 1] * (ms == -INFINITY ? 1.0f : ex2(ms - m)) : 0.0f;
+        l += f[s];
     }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
     for (int e = 0; e < HD / 32; ++e) v[e] = 0.0f;
 #pragma unroll
     for (uint32_t s = 0; s < kKjFew; ++s) {
         if (s < used) {
 #pragma unroll
-            for (int e = 0; e < HD / 32; ++e) v[e] = fmaf(part[s * HD + lane + 32 * e], f[s], v[e]);
+            for (int e = 0; e < HD / 32; ++e) v[e] = fmaf(part[s * HD + lane + 32 * e], f[s] * inv, v[e]);
         }
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     T* out = static_cast<T*>(p.a.out) + row * p.a.out_stride + static_cast<uint64_t>(h) * HD;
 #pragma unroll
-    for (int e = 0; e < HD / 32; ++e) out[lane + 32 * e] = from_f32<T>(v[e] * inv);
+    for (int e = 0; e < HD / 32; ++e) out[lane + 32 * e] = from_f32<T>(v[e]);
     if (p.a.lse && lane == 0) p.a.lse[row * p.a.H + h] = kv8_lse(m, l);
 }
 
@@ -395,8 +402,8 @@ __global__ void __launch_bounds__(kKjThreads) kv8_join_kernel(const Kv8Split p) 
 #pragma unroll
         for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
         for (uint32_t s = lane; s < used; s += 32) {
-            f[s] = ml[2 * s] == -INFINITY ? 1.0f : ex2(ml[2 * s] - m);
-            l += ml[2 * s + 1] * f[s];
+            f[s] = ml[2 * s + 1] * (ml[2 * s] == -INFINITY ? 1.0f : ex2(ml[2 * s] - m));
+            l += f[s];
         }
         l = warp_sum(l);
         if (lane == 0) {
@@ -405,6 +412,7 @@ __global__ void __launch_bounds__(kKjThreads) kv8_join_kernel(const Kv8Split p) 
         }
     }
     __syncthreads();
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     const float* part = p.part + first * HD;
     float v[HD / 32];
 #pragma unroll
@@ -412,18 +420,17 @@ __global__ void __launch_bounds__(kKjThreads) kv8_join_kernel(const Kv8Split p) 
 #pragma unroll 4
     for (uint32_t s = warp; s < used; s += kKjWarps) {
 #pragma unroll
-        for (int e = 0; e < HD / 32; ++e) v[e] = fmaf(part[static_cast<uint64_t>(s) * HD + lane + 32 * e], f[s], v[e]);
+        for (int e = 0; e < HD / 32; ++e) v[e] = fmaf(part[static_cast<uint64_t>(s) * HD + lane + 32 * e], f[s] * inv, v[e]);
     }
 #pragma unroll
     for (int e = 0; e < HD / 32; ++e) o[warp][lane + 32 * e] = v[e];
     __syncthreads();
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     T* out = static_cast<T*>(p.a.out) + row * p.a.out_stride + static_cast<uint64_t>(h) * HD;
     for (int d = threadIdx.x; d < HD; d += kKjThreads) {
         float x = 0.0f;
 #pragma unroll
         for (int w = 0; w < kKjWarps; ++w) x += o[w][d];
-        out[d] = from_f32<T>(x * inv);
+        out[d] = from_f32<T>(x);
     }
 }
 

@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
                 sum *= f;
 #pragma unroll
                 for (int k = 0; k < 32; ++k) {
-                    w[k] = ex2((w[k] - from) + kTcLift);
+                    w[k] = ex2(w[k] - from);
                     sum += w[k];
                 }
 #pragma unroll 1
@@ -687,9 +687,8 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
             tc_fence_after();
         }
         if (mx == -INFINITY && sum < INFINITY) sum = 0.0f;  // nothing seen: what ex2_fma makes of -inf
-        const float ref = mine > 0 ? (slow ? 1.0f : *unit_v) : 0.0f;
-        float mul = used == 1 ? (sum == 0.0f ? 0.0f : ref / sum) : ref;
-        if (poison) mul = NAN;
+        const float ref = mine > 0 ? (slow ? 1.0f : *unit_v) : 0.0f, base = mx - (slow ? 0.0f : kTcLift);
+        const float mul = poison ? NAN : sum == 0.0f ? 0.0f : ref / sum;
         T* out = static_cast<T*>(p.a.out) + at * p.a.out_stride + static_cast<uint64_t>(h) * HD;
         const uint64_t prow = ((static_cast<uint64_t>(seq) * p.a.max_new + i0 + token) * p.a.H + h) * p.splits + split;
         const bool more = RUNS && !slow && mine > kTcRun;
@@ -720,9 +719,9 @@ __global__ void __launch_bounds__(TcShape<HD>::kThreads, 1) kv8_prefill_tc_kerne
         }
         if (live) {
             if (used == 1) {
-                if (p.a.lse) p.a.lse[at * p.a.H + h] = kv8_lse(mx - kTcLift, sum);
+                if (p.a.lse) p.a.lse[at * p.a.H + h] = kv8_lse(base, sum);
             } else {
-                p.part_ml[prow * 2] = mx - kTcLift;
+                p.part_ml[prow * 2] = base;
                 p.part_ml[prow * 2 + 1] = sum;
             }
         }
