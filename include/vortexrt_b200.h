@@ -216,7 +216,8 @@ VRT_API int vrt_q8t_lm_head_argmax(vrt_ctx* ctx, const void* d_packed, uint32_t 
 /* ------------------------------------------------- paged 8-bit KV cache
  * Keys and values of many sequences in pages of VRT_KV8_PAGE tokens, one int8
  * code a value and one fp32 scale for each (page, KV head), K and V apart: a
- * quarter of an fp32 cache.  For the rows x that a page holds so far
+ * quarter of an fp32 cache, and a page of rows (the tail) for each sequence.
+ * For the rows x that a page holds so far
  *     scale = fl32(max|x| / 127),  code = x / scale rounded half to even,
  * so a page's contents depend on its tokens alone and not on the calls that
  * brought them: the rows of a page that is not full are also kept as given
@@ -258,7 +259,13 @@ typedef struct {
  * 0 or p - t < window).  A prefix is thus seen by every query whatever the
  * order and the window (an image's tokens, the first tokens that a sliding
  * window keeps in sight).  s = scale * q.k, then softcap * tanh(s / softcap)
- * when softcap > 0.  A query that sees nothing gives zeros and lse = -inf. */
+ * when softcap > 0.  A query that sees nothing gives zeros and lse = -inf.
+ * Precision: scores, maxima and sums are held in fp32.  Softmax weights of f32
+ * rows are kept to 22 bits, those of f16 and bf16 rows are rounded once to fp16
+ * (half a step, 2^-11); weights below 2^-39 of a row's largest are lost, in
+ * prompts of f16 and bf16 rows those below 2^-28.  Keys and values that a query
+ * does not see have no part in its result, whatever their size, but through the
+ * scale that they share with the others of their page. */
 typedef struct {
     uint32_t heads;          /* query heads: 1 to 8 for each KV head        */
     float scale;
@@ -452,8 +459,9 @@ typedef struct vrt_batch vrt_batch;
 VRT_API int vrt_batch_create(vrt_model* m, uint32_t max_seqs, uint32_t max_positions, int keep_logits,
                              vrt_batch** out);
 /* The same with keys and values held in 8 bits (the paged cache above, fp32
- * rows): a quarter of the cache's bytes, on sliding layers a ring of the
- * window and 512 more tokens.  A value is off by at most 1/254 of the largest
+ * rows): a quarter of the cache's bytes and 32 fp32 rows a sequence and layer
+ * (as much as 128 tokens of codes), on sliding layers a ring of the window and
+ * 512 more tokens.  A value is off by at most 1/254 of the largest
  * of its page and head, so results are those of a slightly rounded cache, not
  * the fp32 cache's. */
 VRT_API int vrt_batch_create_kv8(vrt_model* m, uint32_t max_seqs, uint32_t max_positions, int keep_logits,

@@ -26,7 +26,8 @@
 //
 // Operands: a query row is brought to [2^14, 2^15) by a power of two, then
 // fp16 (exact for f16 and bf16 rows) or, for f32 rows, fp16 + fp16 remainder
-// (22 bits).  Weights are 2^14 exp(s - maximum) in fp16: half a step is 2^-11
+// (22 bits).  Weights are 2^14 exp(s - maximum) in fp16, value codes are stored
+// times 2^-14 against that: half a step is 2^-11
 // of a weight (averaged over the keys below half a step of a 16-bit output),
 // and what falls under fp16's smallest step is 2^-39 of the largest weight;
 // for f32 rows fp16 + fp16 remainder.  The remainders take columns 4..7 when

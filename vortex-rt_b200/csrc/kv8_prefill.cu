@@ -27,7 +27,8 @@ namespace vrt {
 // show; its fp32 sums would have to leave TMEM for every key tile.
 // Bound by latency: f32 rows of 128 dims take 255 registers, so 8 warps an SM,
 // whose tensor pipe is active 37% of the time.  3x512 tokens behind histories
-// to 4096, window 1024 (32/16 heads of 128): 188 us.  Query fragments from
+// to 4096, window 1024 (32/16 heads of 128): 186 us, with spills of 32 bytes (196
+// at 256 dims).  Query fragments from
 // shared memory and 12 warps an SM took 201-221 us.
 constexpr int kKpRows = 64;
 constexpr int kKpThreads = 128;
